@@ -50,6 +50,11 @@ typedef void* md_stream_t; /* hipStream_t */
  * accuracy is gated in tests/test_gpu_fp8.py. */
 #define MD_KV_BF16 0
 #define MD_KV_FP8_E4M3 1
+/* Block-scaled caches (K13 below): uint8 [pages][2][KH][page_size][md_kv_row_bytes()], always with MD_KV_LAYOUT_HND, no per-head scales.
+ * The bytes of a (page, half, kv head) are page_size rows of elements -- D e4m3 bytes, or D / 2 pairs of e2m1 numbers, the even one in the low
+ * four bits -- and behind them page_size rows of D / 32 scale bytes: value = element * 2^(byte - 127), 255 = NaN. */
+#define MD_KV_MXFP8 2
+#define MD_KV_MXFP4 3
 /* Page layout flag, OR-ed into the kv_dtype argument of md_append_paged_kv / md_rope_append (first cache) /
  * md_paged_attn / md_snapkv_select (source cache).  Default (flag absent) is the reference's NHD page
  * cache[page][2][page_size][KH][D]; MD_KV_LAYOUT_HND selects cache[page][2][KH][page_size][D] (flashinfer's other
@@ -157,6 +162,32 @@ int md_paged_attn(const void* q, int64_t q_row_stride, const void* cache, void* 
                   int H, int KH, int D, int page_size, int causal, float sm_scale,
                   int max_pages_per_req, int kv_dtype, const float* k_scale, const float* v_scale,
                   void* workspace, size_t workspace_bytes, md_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * K13  block-scaled KV pages, rows read back, attention with a sliding window (no counterpart in the reference)
+ * md_append_paged_kv and md_rope_append write block-scaled caches too (kv_dtype MD_KV_MXFP8 / MD_KV_MXFP4 | MD_KV_LAYOUT_HND; D 64 or 128,
+ * page_size % 32 == 0).  Scales: per 32 elements of a row the smallest power of two at which no element is off by more than half a step of its
+ * binade (elements round to nearest even, ties too), at least 2^-100; blocks with an infinity or a NaN read as NaN throughout.
+ *
+ * md_kv_row_bytes     bytes of one row of one kv head, scales included (0: no such cache)
+ * md_read_paged_kv    the inverse of md_append_paged_kv, of every kv_dtype: the last n_b = indptr[b+1] - indptr[b] rows of request b as bf16
+ *                     rows indptr[b] ... of k_out / v_out (row strides in elements).  Rows in front of a request's first or outside its pages
+ *                     are left as they were.
+ * md_window_attn      md_paged_attn (causal) of every kv_dtype, where a row at position t sees the positions s <= t with s > t - window or
+ *                     s < sinks (window 0: all up to t).  A row that sees nothing is 0.  What is in a hidden place, infinities and NaN
+ *                     included, has no effect on the rows that it is hidden from.  sm_scale > 0; page_size % 32 == 0; D 64 or 128.
+ * workspace: md_window_attn_workspace_bytes(), 16-byte aligned, of this call alone until it has run.
+ * ---------------------------------------------------------------------- */
+int md_kv_row_bytes(int kv_dtype, int D);
+int md_read_paged_kv(void* k_out, void* v_out, int64_t k_row_stride, int64_t v_row_stride, const int32_t* indptr, const void* cache,
+                     const int32_t* page_indices, const int32_t* page_indptr, const int32_t* last_page_len, int B, int n_max, int KH, int D,
+                     int page_size, int kv_dtype, const float* k_scale, const float* v_scale, md_stream_t stream);
+size_t md_window_attn_workspace_bytes(int B, int n_max, int H, int KH, int D, int max_pages_per_req, int page_size, int kv_dtype, int window,
+                                      int sinks);
+int md_window_attn(const void* q, int64_t q_row_stride, const void* cache, void* out, const int32_t* qo_indptr, const int32_t* page_indices,
+                   const int32_t* page_indptr, const int32_t* last_page_len, int B, int n_max, int H, int KH, int D, int page_size, int window,
+                   int sinks, float sm_scale, int max_pages_per_req, int kv_dtype, const float* k_scale, const float* v_scale, void* workspace,
+                   size_t workspace_bytes, md_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * K6  Attention.gen_draft_kv  (SnapKV select)

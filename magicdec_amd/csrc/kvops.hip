@@ -10,7 +10,7 @@
 // host-precomputed fp32 cos/sin table (on-device powf/sincosf would make it
 // VALU-bound) and un-fused fp32 multiplies/adds so the result is bit-identical
 // to the oracle's numpy arithmetic (x_e*cos - x_o*sin, x_o*cos + x_e*sin).
-#include "md_common.h"
+#include "kvpages.h"
 #include <math.h>
 
 // rows dropped by an append because they fell beyond the request's mapped pages (md_page_overflow_count)
@@ -279,9 +279,13 @@ extern "C" int md_append_paged_kv(const void* k, const void* v, int64_t k_row_st
                  "md_append_paged_kv: k/v/cache must be 16-byte aligned, row strides multiples of 8");
     const int hnd = (kv_dtype & MD_KV_LAYOUT_HND) ? 1 : 0;
     MD_CHECK_ARG((kv_dtype & ~(MD_KV_DTYPE_MASK | MD_KV_LAYOUT_HND)) == 0, "md_append_paged_kv: unknown kv_dtype flags");
+    if (kv_is_mx(kv_dtype & MD_KV_DTYPE_MASK))
+        return md_mx_append(nullptr, k, v, 0, k_row_stride, v_row_stride, nullptr, append_indptr, nullptr, B, n_max, 0, KH, D, nullptr, 0, cache,
+                            page_indices, page_indptr, last_page_len, nullptr, nullptr, nullptr, nullptr, page_size, kv_dtype,
+                            (hipStream_t)stream, "md_append_paged_kv");
     kv_dtype &= MD_KV_DTYPE_MASK;
     MD_CHECK_ARG(kv_dtype == MD_KV_BF16 || (kv_dtype == MD_KV_FP8_E4M3 && k_scale && v_scale),
-                 "md_append_paged_kv: kv_dtype must be MD_KV_BF16 or MD_KV_FP8_E4M3 (with per-head scales)");
+                 "md_append_paged_kv: kv_dtype must be MD_KV_BF16, MD_KV_FP8_E4M3 (with per-head scales), MD_KV_MXFP8 or MD_KV_MXFP4");
     if (kv_dtype == MD_KV_FP8_E4M3)
         hipLaunchKernelGGL((append_kernel<true>), dim3(n_max, B), dim3(256), 0, (hipStream_t)stream, (const bf16_t*)k,
                            (const bf16_t*)v, k_row_stride, v_row_stride, append_indptr, cache, page_indices,
@@ -355,9 +359,13 @@ extern "C" int md_rope_append(const void* q, const void* k, const void* v, int64
                  "md_rope_append: tensors must be 16-byte aligned, row strides multiples of 8");
     const int hnd = (kv_dtype & MD_KV_LAYOUT_HND) ? 1 : 0;
     MD_CHECK_ARG((kv_dtype & ~(MD_KV_DTYPE_MASK | MD_KV_LAYOUT_HND)) == 0, "md_rope_append: unknown kv_dtype flags");
+    if (kv_is_mx(kv_dtype & MD_KV_DTYPE_MASK))
+        return md_mx_append(q, k, v, q_row_stride, k_row_stride, v_row_stride, q_out, indptr, offsets, B, n_max, H, KH, D, cos_sin, max_pos,
+                            cache, page_indices, page_indptr, last_page_len, cache2, page_indices2, page_indptr2, last_page_len2, page_size,
+                            kv_dtype, (hipStream_t)stream, "md_rope_append");
     kv_dtype &= MD_KV_DTYPE_MASK;
     MD_CHECK_ARG(kv_dtype == MD_KV_BF16 || (kv_dtype == MD_KV_FP8_E4M3 && k_scale && v_scale),
-                 "md_rope_append: kv_dtype must be MD_KV_BF16 or MD_KV_FP8_E4M3 (with per-head scales)");
+                 "md_rope_append: kv_dtype must be MD_KV_BF16, MD_KV_FP8_E4M3 (with per-head scales), MD_KV_MXFP8 or MD_KV_MXFP4");
     PageTable t1{cache, page_indices, page_indptr, last_page_len};
     PageTable t2{cache2, page_indices2, page_indptr2, last_page_len2};
     if (kv_dtype == MD_KV_FP8_E4M3)

@@ -1,0 +1,48 @@
+// Attention over the pages of any cache with a sliding window and first tokens that stay visible (md_window_attn): what its kernels share.
+#pragma once
+#include "attn_common.h"
+#include "kvpages.h"
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct WinParams {
+    const bf16_t* q;
+    const unsigned char* cache;
+    bf16_t* out;
+    const int32_t *qo_indptr, *indices, *indptr, *last;
+    float *ws_o, *ws_ml;        // of the splits of a row's keys: weighted sums; reference and weight
+    int64_t q_row_stride;       // elements
+    KvPages g;
+    int B, H, KH, group, page_size, nsplit, n_qgroups;
+    int window, sinks;          // 0: no window
+    float scale_log2;
+    const float *k_scale, *v_scale;      // MD_KV_FP8_E4M3
+};
+
+constexpr float kLowest = -3.402823466e38f;      // reference of a row without a key: finite, so that differences are no NaN
+
+// Bits of the halves of a bf16 pair that are infinite or NaN
+__device__ __forceinline__ unsigned nonfinite_halves(unsigned u) {
+    const unsigned t = ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    return (t - (t >> 15)) | t;
+}
+// 1 (bf16) in the halves that are infinite or NaN and not the infinity of the other sign
+__device__ __forceinline__ unsigned infinite_halves(unsigned u, bool negative) {
+    const unsigned other = negative ? 0x7f80u : 0xff80u;
+    unsigned m = nonfinite_halves(u);
+    if ((u & 0xffffu) == other) m &= 0xffff0000u;
+    if ((u >> 16) == other) m &= 0xffffu;
+    return m & 0x3f803f80u;
+}
+
+// Tiles of KT keys that rows between the positions lo and hi look at: those of the first tokens, then those from the lowest window on
+struct Tiles {
+    int first, w0, count;       // tiles of the first tokens, the window's first tile, tiles in all
+    __device__ __forceinline__ Tiles(int lo, int end, int window, int sinks, int kt) {
+        w0 = window > 0 ? max(lo - window + 1, 0) / kt : 0;
+        first = min(w0, (min(sinks, end) + kt - 1) / kt);
+        count = end > 0 ? first + max((end + kt - 1) / kt - w0, 0) : 0;
+    }
+    __device__ __forceinline__ int at(int i) const { return i < first ? i : i - first + w0; }
+};
+

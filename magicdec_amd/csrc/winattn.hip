@@ -1,0 +1,614 @@
+// md_window_attn: softmax attention of new tokens over paged K / V of any element type, over everything before them or over a sliding window
+// and some first tokens.
+//
+// One wavefront owns a stream of 32-key tiles of one (request, kv head) and up to 32 query rows (query heads of the kv head x new tokens), as
+// S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16:
+//   * the keys of a 16-key block come from memory as the matrix instruction's A operand: lane (row lq, quarter lc) loads the bytes of its own
+//     row that it multiplies, whatever elements of the row they are -- the sum over the elements has any order, the queries are loaded in
+//     the same.  No LDS, no transposition: 8- and 4-bit elements become bf16 in registers, times their block's scale in the conversion.
+//   * the values have to be transposed: converted the same way, they go through a wavefront-private LDS image that ds_read_b64_tr_b16 reads.
+//   * the scores of query lq lie in the lanes of its column, so that the softmax's statistics are per lane, and are the next product's
+//     B operand as they lie.
+// The scales of a tile's 32 keys and 32 values are one load of a wavefront (a lane a row) and go to the lanes that use them by ds_bpermute.
+// The four wavefronts of a workgroup take a (request, kv head, row group)'s tiles in turn and merge through LDS; `nsplit` workgroups share
+// its tiles where there are few of them, merged by a launch behind.
+//
+// What a mask hides may hold anything.  Scores are replaced, not added to.  Values count with weight 0, which is not enough for an infinity or
+// a NaN: in tiles that hide a key from some row, such values are taken out of the image, and what rows that do see them get of them is
+// added by itself (`spread`), from a second and third image of their signs.
+#include "winattn.h"
+
+#include <algorithm>
+
+namespace {
+
+template <int D, int QT>
+__host__ __device__ constexpr int win_wave_lds() {
+    const int image = (D / 16) * kVSub, merge = QT * D * 64 + QT * 128;
+    return ((image > merge ? image : merge) + 255) / 256 * 256;
+}
+
+constexpr int kWaves = 4;
+
+template <int D, int QT, int KIND>
+__global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinParams p) {
+    constexpr int EB = kv_element_bytes(KIND, D);        // bytes of a row's elements
+    constexpr bool MX = kv_is_mx(KIND);
+    constexpr int KS = D / 32, NB = D / 16, SB = D / 32;  // matrix steps of a score, 16-d blocks, scales of a row
+    // keys: a lane's loads of a row, their dwords, elements and matrix steps
+    constexpr int KI = EB >= 64 ? EB / 64 : 1, KW = EB >= 64 ? 4 : EB / 16, EL = D / (4 * KI), SPL = EL / 8;
+    // values: 16-byte pieces of a row, rows of a load, loads
+    constexpr int CH = EB / 16, RPI = 64 / CH, NL = 32 / RPI;
+    // 8 neighbouring lanes write 16-byte halves of 32-byte rows: the upper half of the pieces begin with their second half, so that they
+    // lie in different banks; in the d blocks from 4 on the halves are then the other way round (undone where rows are stored)
+    constexpr bool SWAP = KIND != MD_KV_BF16 && D == 128;
+    constexpr int WAVE_LDS = win_wave_lds<D, QT>();
+    constexpr int NS = KIND == MD_KV_BF16 && QT == 2 && D == 128 ? 1 : 2;        // tiles in flight
+
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63;
+    const int lq = lane & 15, lc = lane >> 4;
+
+    // workgroups of one (request, kv head) differ by multiples of 8: they share an XCD's L2
+    const int nsub = p.n_qgroups * p.nsplit;
+    const int sub = (blockIdx.x >> 3) % nsub, pair = ((blockIdx.x >> 3) / nsub) * 8 + (blockIdx.x & 7);
+    if (pair >= p.B * p.KH) return;
+    const int qg = sub / p.nsplit, split = sub % p.nsplit;
+    const int b = pair / p.KH, kvh = pair % p.KH;
+    const int g = p.group;
+    const int q0 = p.qo_indptr[b], n_b = p.qo_indptr[b + 1] - q0;
+    int pg0, room;
+    const int kv_len = min(kv_len_of(p.indptr, p.last, b, p.page_size, &pg0, &room), room);
+    const int nrows = n_b * g;
+
+    // a lane's query rows see up to lim, and of those up to low only the first tokens
+    int lim[QT], low[QT];
+    int hi = -1, lo = 0x7fffffff;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int R = (qg * QT + qt) * 16 + lq;
+        const bool valid = R < nrows;
+        lim[qt] = valid ? kv_len - n_b + R / g : -1;
+        low[qt] = p.window > 0 ? lim[qt] - p.window : -1;
+        hi = max(hi, lim[qt]);
+        if (valid) lo = min(lo, lim[qt]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        hi = max(hi, __shfl_xor(hi, o));
+        lo = min(lo, __shfl_xor(lo, o));
+    }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int hi_low = p.window > 0 ? hi - p.window : -1;
+    const Tiles tiles(lo, min(hi + 1, kv_len), p.window, p.sinks, 32);
+    const int per = (tiles.count + p.nsplit - 1) / p.nsplit;
+    const int t_begin = split * per, t_end = min(tiles.count, t_begin + per);
+
+    bf16x8 qf[QT][KS];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int R = (qg * QT + qt) * 16 + lq;
+        const int i = R / g, r = R - i * g;
+        const bf16_t* qp = p.q + (int64_t)(q0 + i) * p.q_row_stride + (kvh * g + r) * D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            qf[qt][s] = R < nrows ? *reinterpret_cast<const bf16x8*>(qp + (s / SPL) * 4 * EL + lc * EL + (s % SPL) * 8) : z;
+        }
+    }
+    const float sl2 = KIND == MD_KV_FP8_E4M3 ? p.scale_log2 * p.k_scale[kvh] : p.scale_log2;
+    const float vsc = KIND == MD_KV_FP8_E4M3 ? p.v_scale[kvh] : 1.0f;
+    f32x4 o[QT][NB];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        m[qt] = kLowest;
+        l[qt] = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) o[qt][nb] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    unsigned char* image = smem + wave * WAVE_LDS;
+    const int wrow = lane / CH, wch = lane % CH;
+    const bool swp = SWAP && wch >= CH / 2;
+    const int vra = (lc * 4 + (lq >> 2)) * 32 + (lq & 3) * 8;       // + nb * kVSub, + 512 for the second 16 keys
+
+    struct Staged {
+        unsigned k[2][KI * KW];
+        u32x4 v[NL];
+        unsigned scale;
+    };
+    Staged st[NS];
+    const unsigned koff = (unsigned)(lq * p.g.slot + lc * KW * 4), voff = (unsigned)(wrow * p.g.slot + wch * 16);
+    auto tile_base = [&](int i) {
+        const int pos = tiles.at(i) * 32, page = pos / p.page_size;
+        const int pid = __builtin_amdgcn_readfirstlane(p.indices[pg0 + page]);
+        return p.cache + (int64_t)pid * p.g.page + (int64_t)kvh * p.g.head + (int64_t)(pos - page * p.page_size) * p.g.slot;
+    };
+    auto issue = [&](int i, Staged& s) {
+        const unsigned char* base = tile_base(i);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int k = 0; k < KI; ++k) {
+                const unsigned char* at = base + (int64_t)kb * 16 * p.g.slot + koff + k * 64;
+                if constexpr (KW == 4) {
+                    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s.k[kb][k * 4 + e] = x[e];
+                } else {
+                    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at));
+                    s.k[kb][0] = x[0];
+                    s.k[kb][1] = x[1];
+                }
+            }
+        if constexpr (MX) {
+            const int pos = tiles.at(i) * 32, slot0 = pos % p.page_size;
+            const unsigned char* at = base - (int64_t)slot0 * p.g.slot + p.g.scales + slot0 * SB + (lane >= 32 ? p.g.half : 0) + (lane & 31) * SB;
+            s.scale = SB == 4 ? *reinterpret_cast<const unsigned*>(at) : *reinterpret_cast<const unsigned short*>(at);
+        }
+#pragma unroll
+        for (int j = 0; j < NL; ++j)
+            s.v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)j * RPI * p.g.slot + voff));
+    };
+    auto scale_of = [&](unsigned scales, int row, int block) {       // row 0..31 keys, 32..63 values
+        const unsigned u = (unsigned)__builtin_amdgcn_ds_bpermute(row * 4, (int)scales);
+        return mx_scale((u >> (block * 8)) & 255u);
+    };
+    // a lane's 16 bytes of values as bf16 pairs, in the order of d
+    constexpr int VD = KIND == MD_KV_BF16 ? 4 : KIND == MD_KV_MXFP4 ? 16 : 8;
+    auto values = [&](const u32x4 x, float scale, unsigned (&y)[VD]) {
+        if constexpr (KIND == MD_KV_BF16) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) y[w] = x[w];
+        } else if constexpr (KIND == MD_KV_MXFP4) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                unsigned t[4];
+                mx4_to_bf16(x[w], scale, t);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[4 * w + e] = t[e];
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx8_to_bf16(x[w], scale, y[2 * w], y[2 * w + 1]);
+        }
+    };
+    auto put_values = [&](int j, const unsigned (&y)[VD]) {
+        const int row = (wrow + j * RPI) * 32;
+        if constexpr (KIND == MD_KV_BF16) {
+            *reinterpret_cast<u32x4*>(image + (wch >> 1) * kVSub + row + (wch & 1) * 16) = u32x4{y[0], y[1], y[2], y[3]};
+        } else {
+            constexpr int SUBS = VD / 8;
+#pragma unroll
+            for (int s = 0; s < SUBS; ++s) {
+                unsigned char* at = image + (wch * SUBS + s) * kVSub + row;
+                *reinterpret_cast<u32x4*>(at + (swp ? 16 : 0)) = u32x4{y[8 * s], y[8 * s + 1], y[8 * s + 2], y[8 * s + 3]};
+                *reinterpret_cast<u32x4*>(at + (swp ? 0 : 16)) = u32x4{y[8 * s + 4], y[8 * s + 5], y[8 * s + 6], y[8 * s + 7]};
+            }
+        }
+    };
+    auto value_scale = [&](unsigned scales, int j) {
+        return MX ? scale_of(scales, 32 + wrow + j * RPI, KIND == MD_KV_MXFP4 ? wch : wch >> 1) : 1.0f;
+    };
+    // one wavefront's LDS operations run in order: the compiler has to keep them so, too
+    auto in_order = [&] {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    };
+    auto value_fragment = [&](int nb) {
+        const bf16x4 a = lds_read_tr(image + nb * kVSub + vra), c = lds_read_tr(image + nb * kVSub + 512 + vra);
+        return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    // infinite values and NaN of tile i go to the rows that see them
+    auto spread = [&](int i, const unsigned (&hidden)[QT]) {
+        const unsigned char* base = tile_base(i);
+        const int slot0 = tiles.at(i) * 32 % p.page_size;
+#pragma unroll 1
+        for (int negative = 0; negative < 2; ++negative) {
+            in_order();
+#pragma unroll
+            for (int j = 0; j < NL; ++j) {
+                const int row = wrow + j * RPI;
+                const u32x4 x = *reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)j * RPI * p.g.slot + voff);
+                float scale = 1.0f;
+                if constexpr (MX)
+                    scale = mx_scale(base[p.g.half - (int64_t)slot0 * p.g.slot + p.g.scales + (slot0 + row) * SB + (KIND == MD_KV_MXFP4 ? wch : wch >> 1)]);
+                unsigned y[VD];
+                values(x, scale, y);
+#pragma unroll
+                for (int e = 0; e < VD; ++e) y[e] = infinite_halves(y[e], negative != 0);
+                put_values(j, y);
+            }
+            in_order();
+            const float add = negative ? -INFINITY : INFINITY;
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                bf16x8 seen;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) seen[e] = hidden[qt] >> e & 1 ? (bf16_t)0.f : (bf16_t)1.f;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_fragment(nb), seen, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (n[r] > 0.f) o[qt][nb][r] += add;
+                }
+            }
+        }
+        in_order();
+    };
+
+    auto process = [&](auto more, int i, Staged& s) {
+        const int t = tiles.at(i);
+        const bool need_mask = t * 32 + 31 > lo || (t * 32 <= hi_low && t * 32 + 31 >= p.sinks);
+        bool infinite = false;
+#pragma unroll
+        for (int j = 0; j < NL; ++j) {
+            unsigned y[VD];
+            values(s.v[j], value_scale(s.scale, j), y);
+            if (need_mask) {
+#pragma unroll
+                for (int e = 0; e < VD; ++e) {
+                    const unsigned n = nonfinite_halves(y[e]);
+                    infinite |= n != 0;
+                    y[e] &= ~n;
+                }
+            }
+            put_values(j, y);
+        }
+        f32x4 sc[QT][2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) sc[qt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KI; ++k) {
+                // a lane's piece of a row is one block's, or a half of it
+                const float scale = MX ? scale_of(s.scale, kb * 16 + lq, EL == 32 ? lc : k * 2 + (lc >> 1)) : 1.0f;
+#pragma unroll
+                for (int h = 0; h < SPL; ++h) {
+                    unsigned y[4];
+                    if constexpr (KIND == MD_KV_BF16) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = s.k[kb][k * 4 + e];
+                    } else if constexpr (KIND == MD_KV_MXFP4) {
+                        mx4_to_bf16(s.k[kb][k * KW + h], scale, y);
+                    } else {
+                        mx8_to_bf16(s.k[kb][k * KW + 2 * h], scale, y[0], y[1]);
+                        mx8_to_bf16(s.k[kb][k * KW + 2 * h + 1], scale, y[2], y[3]);
+                    }
+                    const bf16x8 kf = __builtin_bit_cast(bf16x8, u32x4{y[0], y[1], y[2], y[3]});
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        sc[qt][kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[qt][k * SPL + h], sc[qt][kb], 0, 0, 0);
+                }
+            }
+        }
+        if constexpr (decltype(more)::value) {
+            issue(i + NS * kWaves, s);
+        } else {
+            if (i + NS * kWaves < t_end) issue(i + NS * kWaves, s);
+        }
+        in_order();
+
+        bf16x8 pf[QT];
+        unsigned hidden[QT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = sc[qt][e >> 2][e & 3] * sl2;     // rounded here: the largest minus the reference is 0
+            hidden[qt] = 0;
+            if (need_mask) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int pos = t * 32 + (e >> 2) * 16 + lc * 4 + (e & 3);
+                    if (pos > lim[qt] || (pos <= low[qt] && pos >= p.sinks)) {
+                        v[e] = -INFINITY;
+                        hidden[qt] |= 1u << e;
+                    }
+                }
+            }
+            float mx = v[0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, v[e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {         // some row has a new reference
+                const float mnew = fmaxf(m[qt], mx), alpha = __builtin_amdgcn_exp2f(m[qt] - mnew);
+                m[qt] = mnew;
+                l[qt] *= alpha;
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) o[qt][nb] *= alpha;
+            }
+            float ps = 0.f;
+            f32x8 w;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = __builtin_amdgcn_exp2f(v[e] - m[qt]);
+                ps += w[e];
+            }
+            l[qt] += ps;
+            pf[qt] = __builtin_convertvector(w, bf16x8);       // the matrix instruction's operand: weights from 0 to 1, off by 2^-9 of themselves
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const bf16x8 vf = value_fragment(nb);
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) o[qt][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qt], o[qt][nb], 0, 0, 0);
+        }
+        if (need_mask && __builtin_amdgcn_ballot_w64(infinite) != 0) spread(i, hidden);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+
+    // steady state: loads of the tile NS turns on are issued without a condition, so that waits are for the tile at hand alone
+    int i = t_begin + wave;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+        if (i + s * kWaves < t_end) issue(i + s * kWaves, st[s]);
+    for (; i + (2 * NS - 1) * kWaves < t_end; i += NS * kWaves) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) process(std::true_type{}, i + s * kWaves, st[s]);
+    }
+    for (; i < t_end; i += NS * kWaves) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+            if (i + s * kWaves < t_end) process(std::false_type{}, i + s * kWaves, st[s]);
+    }
+
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        l[qt] += __shfl_xor(l[qt], 16);
+        l[qt] += __shfl_xor(l[qt], 32);
+    }
+    __syncthreads();
+    float* mo = reinterpret_cast<float*>(smem + wave * WAVE_LDS);
+    float* mst = mo + QT * D * 16;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mo[(qt * D + nb * 16 + ((SWAP && nb >= 4) ? (lc ^ 2) : lc) * 4 + r) * 16 + lq] = o[qt][nb][r];
+        if (lc == 0) {
+            mst[(qt * 16 + lq) * 2] = m[qt];
+            mst[(qt * 16 + lq) * 2 + 1] = l[qt];
+        }
+    }
+    __syncthreads();
+    constexpr int ROWS = QT * 16;
+    for (int e = tid; e < ROWS * D; e += 64 * kWaves) {
+        const int Rl = e / D, d = e - Rl * D, R = qg * ROWS + Rl;
+        if (R >= nrows) continue;
+        const int qt = Rl >> 4, qq = Rl & 15;
+        float M = kLowest, L = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const float*>(smem + w * WAVE_LDS)[QT * D * 16 + (qt * 16 + qq) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float* ow = reinterpret_cast<const float*>(smem + w * WAVE_LDS);
+            const float* sw = ow + QT * D * 16 + (qt * 16 + qq) * 2;
+            const float a = __builtin_amdgcn_exp2f(sw[0] - M);
+            L += sw[1] * a;
+            acc += ow[(qt * D + d) * 16 + qq] * a;
+        }
+        if (p.nsplit == 1) {
+            const int i = R / g;
+            p.out[((int64_t)(q0 + i) * p.H + kvh * g + R - i * g) * D + d] = f32_to_bf16(L == 0.f ? 0.f : acc * (vsc / L));
+        } else {
+            const int64_t slot = (((int64_t)pair * p.n_qgroups + qg) * p.nsplit + split) * ROWS + Rl;
+            p.ws_o[slot * D + d] = acc;
+            if (d == 0) {
+                p.ws_ml[slot * 2] = M;
+                p.ws_ml[slot * 2 + 1] = L;
+            }
+        }
+    }
+}
+
+// The splits of a row joined: D / 4 lanes a row, SG groups of them share its splits and meet through LDS.
+template <int D, int SG>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WinParams p, int rows) {
+    constexpr int VPR = D / 4, TPR = VPR * SG, RPB = 256 / TPR;
+    __shared__ float s_ml[SG > 1 ? 512 : 1];
+    __shared__ f32x4 s_o[SG > 1 ? 256 : 1];
+    const int tid = threadIdx.x, v = tid % VPR, sg = tid / VPR % SG;
+    const int64_t rowid = (int64_t)blockIdx.x * RPB + tid / TPR;
+    const int Rl = (int)(rowid % rows), item = (int)(rowid / rows);
+    const int pair = item / p.n_qgroups, qg = item % p.n_qgroups, R = qg * rows + Rl;
+    int q0 = 0;
+    bool live = pair < p.B * p.KH;
+    if (live) {
+        q0 = p.qo_indptr[pair / p.KH];
+        live = R < (p.qo_indptr[pair / p.KH + 1] - q0) * p.group;
+    }
+    float M = kLowest, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if (live) {
+        for (int s = sg; s < p.nsplit; s += SG) {
+            const int64_t slot = ((int64_t)item * p.nsplit + s) * rows + Rl;
+            const float ms = p.ws_ml[slot * 2], mn = fmaxf(M, ms);
+            const float a = __builtin_amdgcn_exp2f(M - mn), c = __builtin_amdgcn_exp2f(ms - mn);
+            const f32x4 os = *reinterpret_cast<const f32x4*>(p.ws_o + slot * D + v * 4);
+            L = L * a + p.ws_ml[slot * 2 + 1] * c;
+            acc = acc * a + os * c;
+            M = mn;
+        }
+    }
+    if constexpr (SG > 1) {
+        s_ml[tid * 2] = M;
+        s_ml[tid * 2 + 1] = L;
+        s_o[tid] = acc;
+        __syncthreads();
+        if (sg != 0) return;
+        const float m0 = M;
+#pragma unroll
+        for (int u = 1; u < SG; ++u) M = fmaxf(M, s_ml[(tid + u * VPR) * 2]);
+        const float a = __builtin_amdgcn_exp2f(m0 - M);
+        L *= a;
+        acc *= a;
+#pragma unroll
+        for (int u = 1; u < SG; ++u) {
+            const float c = __builtin_amdgcn_exp2f(s_ml[(tid + u * VPR) * 2] - M);
+            L += s_ml[(tid + u * VPR) * 2 + 1] * c;
+            acc += s_o[tid + u * VPR] * c;
+        }
+    }
+    if (!live) return;
+    const int kvh = pair % p.KH, i = R / p.group;
+    const float inv = L == 0.f ? 0.f : (p.v_scale ? p.v_scale[kvh] : 1.f) / L;
+    if (L == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    *reinterpret_cast<bf16x4*>(p.out + ((int64_t)(q0 + i) * p.H + kvh * p.group + R - i * p.group) * D + v * 4) = __builtin_convertvector(acc * inv, bf16x4);
+}
+
+// How a call's rows and keys lie over workgroups
+struct WinPlan {
+    int qt, rows, n_qgroups, nsplit;
+    size_t slots;
+};
+
+WinPlan window_plan(int B, int n_max, int H, int KH, int max_pages, int page_size, int window, int sinks) {
+    WinPlan pl;
+    const int64_t rows = (int64_t)n_max * (H / KH);
+    pl.qt = rows <= 16 ? 1 : 2;
+    pl.rows = pl.qt * 16;
+    pl.n_qgroups = (int)((rows + pl.rows - 1) / pl.rows);
+    // keys that a row group looks at, at most
+    int64_t keys = (int64_t)max_pages * page_size;
+    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + pl.rows + std::min<int64_t>(sinks, keys));
+    const int64_t tiles = (keys + 31) / 32, groups = (int64_t)B * KH * pl.n_qgroups;
+    pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(groups, 1), tiles / 8, 64}));
+    pl.slots = pl.nsplit > 1 ? (size_t)groups * pl.nsplit * pl.rows : 0;
+    return pl;
+}
+
+template <int D, int QT, int KIND>
+int launch_window(const WinParams& p, int grid, hipStream_t st) {
+    constexpr int lds = kWaves * win_wave_lds<D, QT>();
+    auto k = window_attn_kernel<D, QT, KIND>;
+    if constexpr (lds > 64 * 1024) {
+        static MdPerDeviceOnce once;
+        if (once.first()) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e != hipSuccess) {
+                once.undo();
+                md_set_error("md_window_attn: hipFuncSetAttribute(%d B LDS) failed: %s", lds, hipGetErrorString(e));
+                return MD_ERR_LAUNCH;
+            }
+        }
+    }
+    hipLaunchKernelGGL(k, dim3(grid), dim3(64 * kWaves), lds, st, p);
+    MD_CHECK_LAUNCH("md_window_attn");
+    return MD_OK;
+}
+
+template <int D, int KIND>
+int launch_window_rows(const WinParams& p, int qt, int grid, hipStream_t st) {
+    return qt == 1 ? launch_window<D, 1, KIND>(p, grid, st) : launch_window<D, 2, KIND>(p, grid, st);
+}
+
+template <int D>
+int launch_window_kind(const WinParams& p, int kind, int qt, int grid, hipStream_t st) {
+    switch (kind) {
+        case MD_KV_BF16: return launch_window_rows<D, MD_KV_BF16>(p, qt, grid, st);
+        case MD_KV_FP8_E4M3: return launch_window_rows<D, MD_KV_FP8_E4M3>(p, qt, grid, st);
+        case MD_KV_MXFP8: return launch_window_rows<D, MD_KV_MXFP8>(p, qt, grid, st);
+        default: return launch_window_rows<D, MD_KV_MXFP4>(p, qt, grid, st);
+    }
+}
+
+template <int D>
+void launch_window_merge(const WinParams& p, int rows, hipStream_t st) {
+    const int64_t threads = (int64_t)p.B * p.KH * p.n_qgroups * rows * (D / 4);
+    const int sg = p.nsplit <= 4 ? 1 : 8;
+    const dim3 grid((unsigned)((threads * sg + 255) / 256));
+    if (sg == 1)
+        hipLaunchKernelGGL((window_merge_kernel<D, 1>), grid, dim3(256), 0, st, p, rows);
+    else
+        hipLaunchKernelGGL((window_merge_kernel<D, 8>), grid, dim3(256), 0, st, p, rows);
+}
+
+bool window_shape_ok(int B, int n_max, int H, int KH, int max_pages, int page_size) {
+    return B > 0 && n_max > 0 && KH > 0 && H > 0 && H % KH == 0 && max_pages > 0 && page_size > 0 && page_size % 32 == 0 &&
+           (int64_t)max_pages * page_size < (1 << 30) && (int64_t)n_max * (H / KH) < (1 << 30);
+}
+
+}  // namespace
+
+extern "C" size_t md_window_attn_workspace_bytes(int B, int n_max, int H, int KH, int D, int max_pages_per_req, int page_size, int kv_dtype,
+                                                 int window, int sinks) {
+    (void)kv_dtype;
+    if (!window_shape_ok(B, n_max, H, KH, max_pages_per_req, page_size) || window < 0 || sinks < 0) return 0;
+    return window_plan(B, n_max, H, KH, max_pages_per_req, page_size, window, sinks).slots * ((size_t)D * 4 + 8) + 256;
+}
+
+extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* cache, void* out, const int32_t* qo_indptr,
+                              const int32_t* page_indices, const int32_t* page_indptr, const int32_t* last_page_len, int B, int n_max, int H,
+                              int KH, int D, int page_size, int window, int sinks, float sm_scale, int max_pages_per_req, int kv_dtype,
+                              const float* k_scale, const float* v_scale, void* workspace, size_t workspace_bytes, md_stream_t stream) {
+    MD_CHECK_ARG(q && cache && out && qo_indptr && page_indices && page_indptr && last_page_len, "md_window_attn: null pointer argument");
+    MD_CHECK_ARG(window_shape_ok(B, n_max, H, KH, max_pages_per_req, page_size),
+                 "md_window_attn: bad shape B=%d n_max=%d H=%d KH=%d pages=%d page_size=%d (pages of multiples of 32 rows)", B, n_max, H, KH,
+                 max_pages_per_req, page_size);
+    if (D != 64 && D != 128) {
+        md_set_error("md_window_attn: head_dim %d unsupported (64 or 128)", D);
+        return MD_ERR_UNSUPPORTED;
+    }
+    MD_CHECK_ARG(window >= 0 && sinks >= 0, "md_window_attn: window %d and sinks %d must not be negative", window, sinks);
+    MD_CHECK_ARG(sm_scale > 0.f, "md_window_attn: sm_scale must be > 0");
+    MD_CHECK_ARG(q_row_stride % 8 == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)cache & 15) == 0 && ((uintptr_t)out & 7) == 0,
+                 "md_window_attn: q/cache must be 16-byte aligned with a row stride multiple of 8, out 8-byte aligned");
+    MD_CHECK_ARG((kv_dtype & ~(MD_KV_DTYPE_MASK | MD_KV_LAYOUT_HND)) == 0, "md_window_attn: unknown kv_dtype flags");
+    const bool hnd = (kv_dtype & MD_KV_LAYOUT_HND) != 0;
+    const int kind = kv_dtype & MD_KV_DTYPE_MASK;
+    MD_CHECK_ARG(kind <= MD_KV_MXFP4 && (kind != MD_KV_FP8_E4M3 || (k_scale && v_scale)),
+                 "md_window_attn: kv_dtype must be MD_KV_BF16, MD_KV_FP8_E4M3 (with per-head scales), MD_KV_MXFP8 or MD_KV_MXFP4");
+    MD_CHECK_ARG(hnd || !kv_is_mx(kind), "md_window_attn: block-scaled pages are HND");
+
+    const WinPlan pl = window_plan(B, n_max, H, KH, max_pages_per_req, page_size, window, sinks);
+    const size_t need = pl.slots * ((size_t)D * 4 + 8);
+    if (pl.nsplit > 1 && !(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0)) {
+        md_set_error("md_window_attn: workspace too small or misaligned (%zu < %zu)", workspace_bytes, need);
+        return MD_ERR_WORKSPACE;
+    }
+    const int64_t grid = (int64_t)(B * (int64_t)KH + 7) / 8 * 8 * pl.n_qgroups * pl.nsplit;
+    MD_CHECK_ARG(grid <= 0x7fffffff, "md_window_attn: too many rows for a grid");
+    WinParams p = {};
+    p.q = (const bf16_t*)q;
+    p.cache = (const unsigned char*)cache;
+    p.out = (bf16_t*)out;
+    p.qo_indptr = qo_indptr;
+    p.indices = page_indices;
+    p.indptr = page_indptr;
+    p.last = last_page_len;
+    p.ws_o = (float*)workspace;
+    p.ws_ml = p.ws_o + pl.slots * D;
+    p.q_row_stride = q_row_stride;
+    p.g = kv_pages(kind, KH, D, page_size, hnd);
+    p.B = B;
+    p.H = H;
+    p.KH = KH;
+    p.group = H / KH;
+    p.page_size = page_size;
+    p.nsplit = pl.nsplit;
+    p.n_qgroups = pl.n_qgroups;
+    p.window = window;
+    p.sinks = sinks;
+    p.scale_log2 = sm_scale * 1.4426950408889634f;
+    p.k_scale = kind == MD_KV_FP8_E4M3 ? k_scale : nullptr;
+    p.v_scale = kind == MD_KV_FP8_E4M3 ? v_scale : nullptr;
+    hipStream_t st = (hipStream_t)stream;
+    const int rc = D == 128 ? launch_window_kind<128>(p, kind, pl.qt, (int)grid, st) : launch_window_kind<64>(p, kind, pl.qt, (int)grid, st);
+    if (rc != MD_OK) return rc;
+    if (pl.nsplit > 1) {
+        D == 128 ? launch_window_merge<128>(p, pl.rows, st) : launch_window_merge<64>(p, pl.rows, st);
+        MD_CHECK_LAUNCH("md_window_attn(merge)");
+    }
+    return MD_OK;
+}

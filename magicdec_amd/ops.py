@@ -23,7 +23,10 @@ from ._lib import MagicDecHipError, check  # noqa: F401
 
 PAGE_SIZE = 128
 MD_KV_BF16, MD_KV_FP8_E4M3 = 0, 1      # include/magicdec_hip.h
+MD_KV_MXFP8, MD_KV_MXFP4 = 2, 3
 MD_KV_LAYOUT_HND = 0x100
+MX_DTYPE = torch.uint8                 # of a block-scaled cache
+MX_KINDS = {"mxfp8": MD_KV_MXFP8, "mxfp4": MD_KV_MXFP4}
 FP8_DTYPE = torch.float8_e4m3fn
 KV_LAYOUTS = ("NHD", "HND")
 
@@ -40,10 +43,72 @@ def _kv_geom(kv_cache, kv_layout):
     return kv_cache.shape[2], kv_cache.shape[3], kv_cache.shape[4]
 
 
-def _kv_args(kv_cache, kv_scales, kv_layout="NHD"):
+def mx_kv_cache(num_pages, n_heads, head_dim, kv_dtype, page_size=PAGE_SIZE, device="cuda"):
+    """A block-scaled paged cache of zeros: uint8 [num_pages, 2, n_heads, page_size, row bytes], rows of head_dim elements ("mxfp8": e4m3 bytes,
+    "mxfp4": pairs of e2m1 numbers) and one scale byte for each 32 of them; inside a (page, half, head) all rows' elements come before the
+    scales (include/magicdec_hip.h: MD_KV_MXFP8).  update_kv and rope_append quantise rows as they write them, read_kv and paged_attention
+    read them; kv_layout is "HND" throughout."""
+    return torch.zeros((num_pages, 2, n_heads, page_size, mx_row_bytes(head_dim, kv_dtype)), dtype=MX_DTYPE, device=device)
+
+
+def mx_row_bytes(head_dim, kv_dtype):
+    """Bytes of a kv head's row of a block-scaled cache, its scales included."""
+    if kv_dtype not in MX_KINDS:
+        raise ValueError(f"a block-scaled cache's kv_dtype must be one of {sorted(MX_KINDS)}, got {kv_dtype!r}")
+    if head_dim not in (64, 128):
+        raise ValueError(f"a block-scaled cache needs a head_dim of 64 or 128, got {head_dim}")
+    return (head_dim if kv_dtype == "mxfp8" else head_dim // 2) + head_dim // 32
+
+
+def _is_mx(kv_cache):
+    return kv_cache.dtype == MX_DTYPE
+
+
+def _checked_rows(what, heads, D, *ts):
+    """Rows [rows, heads, D] of bf16 with dense heads and a stride that 16-byte loads of them allow, as many in each."""
+    for t in ts:
+        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (heads, D) or t.shape[0] != ts[0].shape[0] or t.stride(2) != 1 or t.stride(1) != D:
+            raise ValueError(f"{what}: bfloat16 rows [rows, {heads}, {D}] with dense (heads, D) expected, got {t.dtype} {tuple(t.shape)}")
+        if t.stride(0) % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{what}: rows must begin at multiples of 16 bytes")
+
+
+def _checked_table(what, B, qo_indptr, page_indices, page_indptr, last_page_len, offsets=None):
+    """A page table and per-request integers as the kernels read them: int32, contiguous."""
+    for t, n in ((qo_indptr, B + 1), (page_indptr, B + 1), (last_page_len, B), (offsets, B), (page_indices, None)):
+        if t is None:
+            continue
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise TypeError(f"{what}: page tables, lengths and indptr must be contiguous int32 tensors")
+        if n is not None and t.numel() < n:
+            raise ValueError(f"{what}: {t.numel()} integers for {B} requests")
+
+
+def _pages(page_indices, page_indptr):
+    """Page numbers; of requests without a page, memory that is not read in their place."""
+    return _p(page_indices if page_indices.numel() else page_indptr)
+
+
+def _here(what, *ts):
+    """Tensors of the current device, whose current stream the kernels run on."""
+    _gpu(*ts)
+    for t in ts:
+        if t is not None and t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{what}: a tensor of {t.device} while the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _kv_args(kv_cache, kv_scales, kv_layout="NHD", head_dim=None):
     """(kv_dtype | layout flag, k_scale ptr, v_scale ptr) for a paged cache: bf16 caches take no scales, e4m3fn
-    caches need per-kv-head float32 dequantisation scales `(k_scale[KH], v_scale[KH])`."""
+    caches need per-kv-head float32 dequantisation scales `(k_scale[KH], v_scale[KH])`; block-scaled ones (uint8) hold theirs, and their
+    rows' bytes with head_dim say which of the two they are."""
     flag = MD_KV_LAYOUT_HND if kv_layout == "HND" else 0
+    if _is_mx(kv_cache):
+        if kv_layout != "HND" or kv_scales is not None:
+            raise ValueError("a block-scaled KV cache is HND and takes no kv_scales")
+        for name, kind in MX_KINDS.items():
+            if head_dim in (64, 128) and _kv_geom(kv_cache, kv_layout)[2] == mx_row_bytes(head_dim, name):
+                return kind | flag, None, None
+        raise ValueError(f"rows of {kv_cache.shape[4]} bytes are no block-scaled rows of {head_dim} elements (64 or 128)")
     if kv_cache.dtype == torch.bfloat16:
         return MD_KV_BF16 | flag, None, None
     if kv_cache.dtype != FP8_DTYPE:
@@ -88,10 +153,18 @@ def _row_stride(t):
 # ----------------------------------------------------------------------------- K4
 def update_kv(k, v, kv_append_indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, n_max=None,
               kv_scales=None, kv_layout="NHD"):
-    """mylib::update_kv (Engine/utils.py:31-54).  In place on kv_cache."""
+    """mylib::update_kv (Engine/utils.py:31-54).  In place on kv_cache.  A block-scaled cache (mx_kv_cache) gets the rows quantised."""
     _gpu(k, v, kv_cache)
     B = kv_page_indptr.numel() - 1
     page_size, KH, D = _kv_geom(kv_cache, kv_layout)
+    if _is_mx(kv_cache):
+        D = k.shape[-1]
+        _here("update_kv", k, v, kv_cache, kv_append_indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
+        _checked_rows("update_kv", KH, D, k, v)
+        _checked_table("update_kv", B, kv_append_indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
+        if B < 1 or not k.shape[0]:
+            return
+        kv_page_indices = kv_page_indices if kv_page_indices.numel() else kv_page_indptr
     if n_max is None:
         n_max = (k.shape[0] + B - 1) // B if B > 0 else 0
         n_max = max(n_max, 1)
@@ -99,8 +172,28 @@ def update_kv(k, v, kv_append_indptr, kv_cache, kv_page_indices, kv_page_indptr,
     check(lib.md_append_paged_kv(_p(k), _p(v), _row_stride(k), _row_stride(v), _p(_i32(kv_append_indptr)),
                                  _p(kv_cache), _p(_i32(kv_page_indices)), _p(_i32(kv_page_indptr)),
                                  _p(_i32(kv_page_lastlen)), B, n_max, KH, D, page_size,
-                                 *_kv_args(kv_cache, kv_scales, kv_layout), _stream()),
+                                 *_kv_args(kv_cache, kv_scales, kv_layout, D), _stream()),
           "md_append_paged_kv")
+
+
+def read_kv(k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, n_max=None, kv_scales=None, kv_layout="NHD"):
+    """The inverse of update_kv, for every kind of cache: the last indptr[b + 1] - indptr[b] tokens of request b, as bf16, into rows indptr[b] ...
+    of k and v [rows, KH, D] (in place; returns them).  Rows of positions in front of a request's first token or outside its pages stay as they
+    were.  n_max: the most rows of a request (None: as many as there are rows)."""
+    _here("read_kv", k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen)
+    B = kv_page_indptr.numel() - 1
+    page_size, KH, width = _kv_geom(kv_cache, kv_layout)
+    D = k.shape[-1]
+    _checked_rows("read_kv", KH, D, k, v)
+    _checked_table("read_kv", B, indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
+    kv = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    if not _is_mx(kv_cache) and width != D:
+        raise ValueError(f"read_kv: rows of {D} elements of a cache of {width}")
+    if B >= 1 and k.shape[0]:
+        check(_lib.load().md_read_paged_kv(_p(k), _p(v), k.stride(0), v.stride(0), _p(indptr), _p(kv_cache),
+                                           _pages(kv_page_indices, kv_page_indptr), _p(kv_page_indptr), _p(kv_page_lastlen), B, k.shape[0] if n_max is None else n_max, KH, D, page_size,
+                                           *kv, _stream()), "md_read_paged_kv")
+    return k, v
 
 
 def page_overflow_count(reset=True):
@@ -151,11 +244,27 @@ def rope_append(q, k, v, indptr, offsets, table: RopeTable, kv_cache, page_indic
                 kv_cache2=None, page_indices2=None, page_indptr2=None, last_page_len2=None, n_max=None,
                 kv_scales=None, kv_layout="NHD"):
     """Fused mylib::rope + mylib::update_kv (+ second cache for self-spec verify).  Returns rotated q.
-    kv_cache may be fp8 (with kv_scales) and/or HND (kv_layout); kv_cache2 is always bf16 NHD."""
+    kv_cache may be fp8 (with kv_scales) and/or HND (kv_layout), or block-scaled (mx_kv_cache); kv_cache2 is always bf16 NHD."""
     _gpu(q, k, v, kv_cache, kv_cache2)
     B = indptr.numel() - 1
     H, D = q.shape[1], q.shape[2]
     KH = k.shape[1]
+    if _is_mx(kv_cache):
+        _here("rope_append", q, k, v, indptr, offsets, table.table, kv_cache, page_indices, page_indptr, last_page_len, kv_cache2, page_indices2,
+              page_indptr2, last_page_len2)
+        _checked_rows("rope_append", H, D, q)
+        _checked_rows("rope_append", _kv_geom(kv_cache, kv_layout)[1], D, k, v)
+        _checked_table("rope_append", B, indptr, page_indices, page_indptr, last_page_len, offsets)
+        if q.shape[0] != k.shape[0] or table.head_dim != D:
+            raise ValueError("rope_append: as many rows of q as of k and a table of their head size expected")
+        if kv_cache2 is not None:
+            _checked_table("rope_append", B, indptr, page_indices2, page_indptr2, last_page_len2)
+            if (kv_cache2.dtype != torch.bfloat16 or not kv_cache2.is_contiguous()
+                    or kv_cache2.shape[1:] != (2, kv_cache.shape[3], KH, D)):
+                raise ValueError("rope_append: the second cache must be bfloat16 [pages, 2, page, KH, D] with the first one's page size")
+        if B < 1 or not q.shape[0]:
+            return torch.empty_like(q, memory_format=torch.contiguous_format)
+        page_indices = page_indices if page_indices.numel() else page_indptr
     if n_max is None:
         n_max = max((q.shape[0] + B - 1) // B, 1)
     q_out = torch.empty((q.shape[0], H, D), dtype=q.dtype, device=q.device)
@@ -164,7 +273,7 @@ def rope_append(q, k, v, indptr, offsets, table: RopeTable, kv_cache, page_indic
                              _p(_i32(indptr)), _p(_i32(offsets)), B, n_max, H, KH, D, _p(table.table), table.max_pos,
                              _p(kv_cache), _p(_i32(page_indices)), _p(_i32(page_indptr)), _p(_i32(last_page_len)),
                              _p(kv_cache2), _p(page_indices2), _p(page_indptr2), _p(last_page_len2),
-                             _kv_geom(kv_cache, kv_layout)[0], *_kv_args(kv_cache, kv_scales, kv_layout), _stream()),
+                             _kv_geom(kv_cache, kv_layout)[0], *_kv_args(kv_cache, kv_scales, kv_layout, D), _stream()),
           "md_rope_append")
     return q_out
 
@@ -194,10 +303,16 @@ class AttnWorkspace:
 
 def paged_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, n_max, max_pages_per_req,
                     workspace: AttnWorkspace, causal=True, sm_scale=None, out=None, kv_scales=None,
-                    kv_layout="NHD"):
+                    kv_layout="NHD", window=None, sinks=0):
     """mylib::target_decode / target_prefill / draft_decode / draft_prefill
     (Engine/SnapKV/backend.py:56-107): flashinfer BatchPrefillWithPagedKVCacheWrapper.run with the
-    plan() arguments passed explicitly."""
+    plan() arguments passed explicitly.
+
+    window: a row at position t sees the positions s <= t with s > t - window or s < sinks (None: all).  With a window, and over block-scaled
+    caches (mx_kv_cache), the attention is causal."""
+    if window is not None or _is_mx(kv_cache):
+        return _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, n_max, max_pages_per_req, workspace, causal,
+                                 sm_scale, out, kv_scales, kv_layout, window, sinks)
     _gpu(q, kv_cache)
     B = page_indptr.numel() - 1
     H, D = q.shape[1], q.shape[2]
@@ -215,6 +330,37 @@ def paged_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page
                             *_kv_args(kv_cache, kv_scales, kv_layout),
                             _p(ws), ws.numel(), _stream()),
           "md_paged_attn")
+    return out
+
+
+def _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, n_max, max_pages_per_req, workspace, causal, sm_scale, out,
+                      kv_scales, kv_layout, window, sinks):
+    what = "paged_attention"
+    _here(what, q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, out)
+    B = page_indptr.numel() - 1
+    page_size, KH, width = _kv_geom(kv_cache, kv_layout)
+    _, H, D = q.shape
+    _checked_rows(what, H, D, q)
+    _checked_table(what, B, qo_indptr, page_indices, page_indptr, last_page_len)
+    kv = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    if not causal:
+        raise ValueError(f"{what}: attention with a window or over a block-scaled cache is causal")
+    if H % KH or (not _is_mx(kv_cache) and width != D):
+        raise ValueError(f"{what}: {H} query heads of {D} over {KH} kv heads of {width}")
+    if (window is not None and window < 1) or sinks < 0:
+        raise ValueError(f"{what}: window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be a contiguous tensor like q")
+    if B < 1 or not q.shape[0]:
+        return out
+    window, sinks = 0 if window is None else min(window, 1 << 30), min(sinks, 1 << 30)
+    lib = _lib.load()
+    ws = workspace.get(lib.md_window_attn_workspace_bytes(B, n_max, H, KH, D, max_pages_per_req, page_size, kv[0], window, sinks))
+    check(lib.md_window_attn(_p(q), q.stride(0), _p(kv_cache), _p(out), _p(qo_indptr), _pages(page_indices, page_indptr), _p(page_indptr), _p(last_page_len), B,
+                             n_max, H, KH, D, page_size, window, sinks, float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale),
+                             max_pages_per_req, *kv, _p(ws), ws.numel(), _stream()), "md_window_attn")
     return out
 
 
