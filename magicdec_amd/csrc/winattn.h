@@ -46,3 +46,8 @@ struct Tiles {
     __device__ __forceinline__ int at(int i) const { return i < first ? i : i - first + w0; }
 };
 
+// winprompt.hip, an object each: calls of more than 32 rows, in workgroups of nw (4 or 8) wavefronts of 32
+int md_window_prompt_0(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_BF16
+int md_window_prompt_1(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_FP8_E4M3
+int md_window_prompt_2(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_MXFP8
+int md_window_prompt_3(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_MXFP4

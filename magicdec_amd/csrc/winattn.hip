@@ -469,21 +469,23 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinParams p, in
 
 // How a call's rows and keys lie over workgroups
 struct WinPlan {
-    int qt, rows, n_qgroups, nsplit;
+    int nw;                 // wavefronts of a workgroup of winprompt.hip, 0: the kernel above
+    int rows, n_qgroups, nsplit;
     size_t slots;
 };
 
 WinPlan window_plan(int B, int n_max, int H, int KH, int max_pages, int page_size, int window, int sinks) {
     WinPlan pl;
     const int64_t rows = (int64_t)n_max * (H / KH);
-    pl.qt = rows <= 16 ? 1 : 2;
-    pl.rows = pl.qt * 16;
+    pl.nw = rows <= 32 ? 0 : rows >= 256 ? 8 : 4;
+    pl.rows = pl.nw ? pl.nw * 32 : rows <= 16 ? 16 : 32;
     pl.n_qgroups = (int)((rows + pl.rows - 1) / pl.rows);
     // keys that a row group looks at, at most
     int64_t keys = (int64_t)max_pages * page_size;
     if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + pl.rows + std::min<int64_t>(sinks, keys));
-    const int64_t tiles = (keys + 31) / 32, groups = (int64_t)B * KH * pl.n_qgroups;
-    pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(groups, 1), tiles / 8, 64}));
+    const int64_t groups = (int64_t)B * KH * pl.n_qgroups;
+    pl.nsplit = pl.nw ? (int)std::max<int64_t>(1, std::min<int64_t>({256 / groups, keys / 384, 32}))
+                      : (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, keys / 256, 64}));
     pl.slots = pl.nsplit > 1 ? (size_t)groups * pl.nsplit * pl.rows : 0;
     return pl;
 }
@@ -509,17 +511,26 @@ int launch_window(const WinParams& p, int grid, hipStream_t st) {
 }
 
 template <int D, int KIND>
-int launch_window_rows(const WinParams& p, int qt, int grid, hipStream_t st) {
-    return qt == 1 ? launch_window<D, 1, KIND>(p, grid, st) : launch_window<D, 2, KIND>(p, grid, st);
+int launch_window_rows(const WinParams& p, int rows, int grid, hipStream_t st) {
+    return rows == 16 ? launch_window<D, 1, KIND>(p, grid, st) : launch_window<D, 2, KIND>(p, grid, st);
 }
 
 template <int D>
-int launch_window_kind(const WinParams& p, int kind, int qt, int grid, hipStream_t st) {
+int launch_window_kind(const WinParams& p, int kind, int rows, int grid, hipStream_t st) {
     switch (kind) {
-        case MD_KV_BF16: return launch_window_rows<D, MD_KV_BF16>(p, qt, grid, st);
-        case MD_KV_FP8_E4M3: return launch_window_rows<D, MD_KV_FP8_E4M3>(p, qt, grid, st);
-        case MD_KV_MXFP8: return launch_window_rows<D, MD_KV_MXFP8>(p, qt, grid, st);
-        default: return launch_window_rows<D, MD_KV_MXFP4>(p, qt, grid, st);
+        case MD_KV_BF16: return launch_window_rows<D, MD_KV_BF16>(p, rows, grid, st);
+        case MD_KV_FP8_E4M3: return launch_window_rows<D, MD_KV_FP8_E4M3>(p, rows, grid, st);
+        case MD_KV_MXFP8: return launch_window_rows<D, MD_KV_MXFP8>(p, rows, grid, st);
+        default: return launch_window_rows<D, MD_KV_MXFP4>(p, rows, grid, st);
+    }
+}
+
+int launch_window_prompt(const WinParams& p, int kind, int D, int nw, int grid, hipStream_t st) {
+    switch (kind) {
+        case MD_KV_BF16: return md_window_prompt_0(p, D, nw, grid, st);
+        case MD_KV_FP8_E4M3: return md_window_prompt_1(p, D, nw, grid, st);
+        case MD_KV_MXFP8: return md_window_prompt_2(p, D, nw, grid, st);
+        default: return md_window_prompt_3(p, D, nw, grid, st);
     }
 }
 
@@ -604,7 +615,8 @@ extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* c
     p.k_scale = kind == MD_KV_FP8_E4M3 ? k_scale : nullptr;
     p.v_scale = kind == MD_KV_FP8_E4M3 ? v_scale : nullptr;
     hipStream_t st = (hipStream_t)stream;
-    const int rc = D == 128 ? launch_window_kind<128>(p, kind, pl.qt, (int)grid, st) : launch_window_kind<64>(p, kind, pl.qt, (int)grid, st);
+    const int rc = pl.nw ? launch_window_prompt(p, kind, D, pl.nw, (int)grid, st)
+                   : D == 128 ? launch_window_kind<128>(p, kind, pl.rows, (int)grid, st) : launch_window_kind<64>(p, kind, pl.rows, (int)grid, st);
     if (rc != MD_OK) return rc;
     if (pl.nsplit > 1) {
         D == 128 ? launch_window_merge<128>(p, pl.rows, st) : launch_window_merge<64>(p, pl.rows, st);
