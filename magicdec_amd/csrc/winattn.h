@@ -21,6 +21,20 @@ struct WinParams {
 
 constexpr float kLowest = -3.402823466e38f;      // reference of a row without a key: finite, so that differences are no NaN
 
+// Largest of lanes l and l ^ 16, of l and l ^ 32: swaps of 16 and of 32 lanes, no LDS
+__device__ __forceinline__ float max_over_16(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float max_over_32(float x) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
 // Bits of the halves of a bf16 pair that are infinite or NaN
 __device__ __forceinline__ unsigned nonfinite_halves(unsigned u) {
     const unsigned t = ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
@@ -44,6 +58,34 @@ struct Tiles {
         count = end > 0 ? first + max((end + kt - 1) / kt - w0, 0) : 0;
     }
     __device__ __forceinline__ int at(int i) const { return i < first ? i : i - first + w0; }
+};
+
+// Where a wavefront is in a request's pages: the numbers of 64 of them, one a lane, so that a tile waits for no number of its page.
+struct PageCursor {
+    const int32_t* list;
+    int count, size, base, ids;          // pages of the request, rows of a page; first page that `ids` holds
+    int first, page, slot;               // position, number in the request, and row in it
+    __device__ __forceinline__ PageCursor(const WinParams& p, int pg0, int room)
+        : list(p.indices + pg0), count(room / p.page_size), size(p.page_size), base(-64), ids(0), first(0), page(0), slot(0) {}
+    // to position pos, of a page of the request; anywhere, and cheaply where it is less than two pages on
+    __device__ __forceinline__ void seek(int pos) {
+        slot = pos - first;
+        if (slot < 0 || slot >= 2 * size) {
+            page = pos / size;
+            first = page * size;
+            slot = pos - first;
+        } else if (slot >= size) {
+            ++page;
+            first += size;
+            slot -= size;
+        }
+        if (page < base || page >= base + 64) {
+            base = page;
+            ids = list[min(page + (int)(threadIdx.x & 63), count - 1)];
+            asm volatile("" : "+v"(ids));         // waited for here: behind the branch it would be in every tile
+        }
+    }
+    __device__ __forceinline__ int64_t id() const { return __builtin_amdgcn_readlane(ids, page - base); }
 };
 
 // winprompt.hip, an object each: calls of more than 32 rows, in workgroups of nw (4 or 8) wavefronts of 32

@@ -43,7 +43,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     // lie in different banks; in the d blocks from 4 on the halves are then the other way round (undone where rows are stored)
     constexpr bool SWAP = KIND != MD_KV_BF16 && D == 128;
     constexpr int WAVE_LDS = win_wave_lds<D, QT>();
-    constexpr int NS = KIND == MD_KV_BF16 && QT == 2 && D == 128 ? 1 : 2;        // tiles in flight
+    // tiles in flight: with two row tiles of 128 a second one spills (mxfp8, 64 requests of 8 100 keys, 20 rows a kv head: 223 us, 198 with one)
+    constexpr int NS = QT == 2 && D == 128 && KIND != MD_KV_MXFP4 ? 1 : 2;
 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x;
@@ -123,10 +124,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     };
     Staged st[NS];
     const unsigned koff = (unsigned)(lq * p.g.slot + lc * KW * 4), voff = (unsigned)(wrow * p.g.slot + wch * 16);
+    const int64_t soff = (lane >= 32 ? p.g.half : 0) + (lane & 31) * SB;
+    PageCursor at(p, pg0, room);
     auto tile_base = [&](int i) {
-        const int pos = tiles.at(i) * 32, page = pos / p.page_size;
-        const int pid = __builtin_amdgcn_readfirstlane(p.indices[pg0 + page]);
-        return p.cache + (int64_t)pid * p.g.page + (int64_t)kvh * p.g.head + (int64_t)(pos - page * p.page_size) * p.g.slot;
+        at.seek(tiles.at(i) * 32);
+        return p.cache + at.id() * p.g.page + (int64_t)kvh * p.g.head + (int64_t)at.slot * p.g.slot;
     };
     auto issue = [&](int i, Staged& s) {
         const unsigned char* base = tile_base(i);
@@ -134,21 +136,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int k = 0; k < KI; ++k) {
-                const unsigned char* at = base + (int64_t)kb * 16 * p.g.slot + koff + k * 64;
+                const unsigned char* from = base + (int64_t)kb * 16 * p.g.slot + koff + k * 64;
                 if constexpr (KW == 4) {
-                    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at));
+                    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(from));
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s.k[kb][k * 4 + e] = x[e];
                 } else {
-                    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(at));
+                    const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(from));
                     s.k[kb][0] = x[0];
                     s.k[kb][1] = x[1];
                 }
             }
         if constexpr (MX) {
-            const int pos = tiles.at(i) * 32, slot0 = pos % p.page_size;
-            const unsigned char* at = base - (int64_t)slot0 * p.g.slot + p.g.scales + slot0 * SB + (lane >= 32 ? p.g.half : 0) + (lane & 31) * SB;
-            s.scale = SB == 4 ? *reinterpret_cast<const unsigned*>(at) : *reinterpret_cast<const unsigned short*>(at);
+            const unsigned char* from = base - (int64_t)at.slot * (EB - SB) + p.g.scales + soff;
+            s.scale = SB == 4 ? *reinterpret_cast<const unsigned*>(from) : *reinterpret_cast<const unsigned short*>(from);
         }
 #pragma unroll
         for (int j = 0; j < NL; ++j)
@@ -207,7 +208,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     // infinite values and NaN of tile i go to the rows that see them
     auto spread = [&](int i, const unsigned (&hidden)[QT]) {
         const unsigned char* base = tile_base(i);
-        const int slot0 = tiles.at(i) * 32 % p.page_size;
 #pragma unroll 1
         for (int negative = 0; negative < 2; ++negative) {
             in_order();
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
                 const u32x4 x = *reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)j * RPI * p.g.slot + voff);
                 float scale = 1.0f;
                 if constexpr (MX)
-                    scale = mx_scale(base[p.g.half - (int64_t)slot0 * p.g.slot + p.g.scales + (slot0 + row) * SB + (KIND == MD_KV_MXFP4 ? wch : wch >> 1)]);
+                    scale = mx_scale(base[p.g.half - (int64_t)at.slot * (EB - SB) + p.g.scales + row * SB + (KIND == MD_KV_MXFP4 ? wch : wch >> 1)]);
                 unsigned y[VD];
                 values(x, scale, y);
 #pragma unroll
@@ -305,20 +305,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
             for (int e = 0; e < 8; ++e) v[e] = sc[qt][e >> 2][e & 3] * sl2;     // rounded here: the largest minus the reference is 0
             hidden[qt] = 0;
             if (need_mask) {
+                // a branch of the wavefront: volatile, or every tile would compare and select
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int pos = t * 32 + (e >> 2) * 16 + lc * 4 + (e & 3);
-                    if (pos > lim[qt] || (pos <= low[qt] && pos >= p.sinks)) {
-                        v[e] = -INFINITY;
-                        hidden[qt] |= 1u << e;
-                    }
+                    const bool out = pos > lim[qt] || (pos <= low[qt] && pos >= p.sinks);
+                    float x = out ? -INFINITY : v[e];
+                    asm volatile("" : "+v"(x));
+                    v[e] = x;
+                    hidden[qt] |= (unsigned)out << e;
                 }
             }
             float mx = v[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, v[e]);
-            mx = fmaxf(mx, __shfl_xor(mx, 16));
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            mx = max_over_32(max_over_16(mx));
             if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {         // some row has a new reference
                 const float mnew = fmaxf(m[qt], mx), alpha = __builtin_amdgcn_exp2f(m[qt] - mnew);
                 m[qt] = mnew;

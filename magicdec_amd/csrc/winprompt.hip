@@ -107,10 +107,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     const unsigned goff = (unsigned)(wrow * p.g.slot + wch * 16);
     u32x4 kreg[NLW], vreg[NLW];
     unsigned kscale[NLW], vscale[NLW];
+    PageCursor at(p, pg0, room);
     auto tile_base = [&](int pos) {
-        const int page = pos / p.page_size;
-        const int pid = __builtin_amdgcn_readfirstlane(p.indices[pg0 + page]);
-        return p.cache + (int64_t)pid * p.g.page + (int64_t)kvh * p.g.head;
+        at.seek(pos);
+        return p.cache + at.id() * p.g.page + (int64_t)kvh * p.g.head;
     };
     auto load = [&](const unsigned char* head, int slot0, int s, u32x4& x, unsigned& scale) {
         const int first = (wave + NW * s) * RPI;
@@ -118,8 +118,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
         if constexpr (MX) scale = head[p.g.scales + (slot0 + first + wrow) * SB + wch * PIECE / 32];
     };
     auto issue = [&](int i) {
-        const int pos = tiles.at(i) * KT, slot0 = pos % p.page_size;
-        const unsigned char* head = tile_base(pos);
+        const unsigned char* head = tile_base(tiles.at(i) * KT);
+        const int slot0 = at.slot;
 #pragma unroll
         for (int s = 0; s < NLW; ++s)
             if (wave + NW * s < NL) {
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
         for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kg][r]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32)) * sl2;
+        mx = max_over_32(mx) * sl2;
         if (__builtin_amdgcn_ballot_w64(mx > m) != 0) {
             const float mnew = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mnew);
             m = mnew;
@@ -269,8 +269,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     };
     // infinite values and NaN of a tile to the rows that see them: by images of their signs in the values' place
     auto spread = [&](int i, unsigned char* img) {
-        const int pos0 = tiles.at(i) * KT, slot0 = pos0 % p.page_size;
+        const int pos0 = tiles.at(i) * KT;
         const unsigned char* head = tile_base(pos0) + p.g.half;
+        const int slot0 = at.slot;
 #pragma unroll 1
         for (int negative = 0; negative < 2; ++negative) {
             __syncthreads();

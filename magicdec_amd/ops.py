@@ -60,41 +60,55 @@ def mx_row_bytes(head_dim, kv_dtype):
     return (head_dim if kv_dtype == "mxfp8" else head_dim // 2) + head_dim // 32
 
 
+_MX_ROWS = {(D, mx_row_bytes(D, name)): kind for name, kind in MX_KINDS.items() for D in (64, 128)}
+
+
 def _is_mx(kv_cache):
-    return kv_cache.dtype == MX_DTYPE
+    return kv_cache.dtype is MX_DTYPE
 
 
-def _checked_rows(what, heads, D, *ts):
-    """Rows [rows, heads, D] of bf16 with dense heads and a stride that 16-byte loads of them allow, as many in each."""
-    for t in ts:
-        if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (heads, D) or t.shape[0] != ts[0].shape[0] or t.stride(2) != 1 or t.stride(1) != D:
-            raise ValueError(f"{what}: bfloat16 rows [rows, {heads}, {D}] with dense (heads, D) expected, got {t.dtype} {tuple(t.shape)}")
-        if t.stride(0) % 8 or t.data_ptr() % 16:
-            raise ValueError(f"{what}: rows must begin at multiples of 16 bytes")
+# The checks of calls that a step makes: attributes of a tensor that cost least, each asked for once.  A step's calls are as short for the GPU as
+# they are for the host (append and read_kv of 256 rows: 7 us of kernels; 46 us of the host with torch.cuda.current_stream, shapes and
+# ctypes objects for every argument, 25 so).
+def _here(what, first, *ts):
+    """The current device, on which all these tensors (or None) have to be: the kernels run on its current stream."""
+    if not first.is_cuda:
+        _gpu(first)
+    cur = torch._C._cuda_getDevice()
+    for t in (first, *ts):
+        if t is not None and t.get_device() != cur:
+            _gpu(t)
+            raise ValueError(f"{what}: a tensor of {t.device} while the current device is cuda:{cur}")
+    return cur
 
 
-def _checked_table(what, B, qo_indptr, page_indices, page_indptr, last_page_len, offsets=None):
-    """A page table and per-request integers as the kernels read them: int32, contiguous."""
-    for t, n in ((qo_indptr, B + 1), (page_indptr, B + 1), (last_page_len, B), (offsets, B), (page_indices, None)):
-        if t is None:
-            continue
-        if t.dtype != torch.int32 or not t.is_contiguous():
+def _rows_of(what, t, heads, D):
+    """How many rows [rows, heads, D] of bf16 with dense heads, at strides that 16-byte loads of them allow."""
+    n, h, d = t.shape
+    s, sh, sd = t.stride()
+    if t.dtype is not torch.bfloat16 or h != heads or d != D or sd != 1 or sh != D:
+        raise ValueError(f"{what}: bfloat16 rows [rows, {heads}, {D}] with dense (heads, D) expected, got {t.dtype} {tuple(t.shape)}")
+    if s % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{what}: rows must begin at multiples of 16 bytes")
+    return n
+
+
+def _table_of(what, indptr, page_indices, page_indptr, last_page_len, offsets=None):
+    """How many requests a page table, with the rows' indptr and offsets, has: int32, contiguous."""
+    for t in (indptr, page_indices, page_indptr, last_page_len):
+        if t.dtype is not torch.int32 or not t.is_contiguous():
             raise TypeError(f"{what}: page tables, lengths and indptr must be contiguous int32 tensors")
-        if n is not None and t.numel() < n:
-            raise ValueError(f"{what}: {t.numel()} integers for {B} requests")
+    B = page_indptr.numel() - 1
+    if indptr.numel() <= B or last_page_len.numel() < B:
+        raise ValueError(f"{what}: {indptr.numel()} and {last_page_len.numel()} integers for {B} requests")
+    if offsets is not None and (offsets.dtype is not torch.int32 or not offsets.is_contiguous() or offsets.numel() < B):
+        raise TypeError(f"{what}: offsets must be contiguous int32, one a request")
+    return B
 
 
 def _pages(page_indices, page_indptr):
     """Page numbers; of requests without a page, memory that is not read in their place."""
-    return _p(page_indices if page_indices.numel() else page_indptr)
-
-
-def _here(what, *ts):
-    """Tensors of the current device, whose current stream the kernels run on."""
-    _gpu(*ts)
-    for t in ts:
-        if t is not None and t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{what}: a tensor of {t.device} while the current device is cuda:{torch.cuda.current_device()}")
+    return (page_indices if page_indices.numel() else page_indptr).data_ptr()
 
 
 def _kv_args(kv_cache, kv_scales, kv_layout="NHD", head_dim=None):
@@ -105,9 +119,9 @@ def _kv_args(kv_cache, kv_scales, kv_layout="NHD", head_dim=None):
     if _is_mx(kv_cache):
         if kv_layout != "HND" or kv_scales is not None:
             raise ValueError("a block-scaled KV cache is HND and takes no kv_scales")
-        for name, kind in MX_KINDS.items():
-            if head_dim in (64, 128) and _kv_geom(kv_cache, kv_layout)[2] == mx_row_bytes(head_dim, name):
-                return kind | flag, None, None
+        kind = _MX_ROWS.get((head_dim, kv_cache.shape[4]))
+        if kind is not None:
+            return kind | flag, None, None
         raise ValueError(f"rows of {kv_cache.shape[4]} bytes are no block-scaled rows of {head_dim} elements (64 or 128)")
     if kv_cache.dtype == torch.bfloat16:
         return MD_KV_BF16 | flag, None, None
@@ -154,17 +168,11 @@ def _row_stride(t):
 def update_kv(k, v, kv_append_indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, n_max=None,
               kv_scales=None, kv_layout="NHD"):
     """mylib::update_kv (Engine/utils.py:31-54).  In place on kv_cache.  A block-scaled cache (mx_kv_cache) gets the rows quantised."""
+    if _is_mx(kv_cache):
+        return _update_kv_mx(k, v, kv_append_indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, n_max, kv_scales, kv_layout)
     _gpu(k, v, kv_cache)
     B = kv_page_indptr.numel() - 1
     page_size, KH, D = _kv_geom(kv_cache, kv_layout)
-    if _is_mx(kv_cache):
-        D = k.shape[-1]
-        _here("update_kv", k, v, kv_cache, kv_append_indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
-        _checked_rows("update_kv", KH, D, k, v)
-        _checked_table("update_kv", B, kv_append_indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
-        if B < 1 or not k.shape[0]:
-            return
-        kv_page_indices = kv_page_indices if kv_page_indices.numel() else kv_page_indptr
     if n_max is None:
         n_max = (k.shape[0] + B - 1) // B if B > 0 else 0
         n_max = max(n_max, 1)
@@ -172,27 +180,46 @@ def update_kv(k, v, kv_append_indptr, kv_cache, kv_page_indices, kv_page_indptr,
     check(lib.md_append_paged_kv(_p(k), _p(v), _row_stride(k), _row_stride(v), _p(_i32(kv_append_indptr)),
                                  _p(kv_cache), _p(_i32(kv_page_indices)), _p(_i32(kv_page_indptr)),
                                  _p(_i32(kv_page_lastlen)), B, n_max, KH, D, page_size,
-                                 *_kv_args(kv_cache, kv_scales, kv_layout, D), _stream()),
+                                 *_kv_args(kv_cache, kv_scales, kv_layout), _stream()),
           "md_append_paged_kv")
+
+
+def _update_kv_mx(k, v, indptr, kv_cache, page_indices, page_indptr, last_page_len, n_max, kv_scales, kv_layout):
+    what = "update_kv"
+    cur = _here(what, k, v, kv_cache, indptr, page_indices, page_indptr, last_page_len)
+    page_size, KH, _ = _kv_geom(kv_cache, kv_layout)
+    D = k.shape[-1]
+    kind, _, _ = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    rows, B = _rows_of(what, k, KH, D), _table_of(what, indptr, page_indices, page_indptr, last_page_len)
+    if _rows_of(what, v, KH, D) != rows:
+        raise ValueError(f"{what}: {rows} rows of k and {v.shape[0]} of v")
+    if B < 1 or not rows:
+        return
+    check(_lib.load().md_append_paged_kv(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), indptr.data_ptr(), kv_cache.data_ptr(),
+                                         _pages(page_indices, page_indptr), page_indptr.data_ptr(), last_page_len.data_ptr(), B,
+                                         rows if n_max is None else n_max, KH, D, page_size, kind, None, None,
+                                         torch._C._cuda_getCurrentRawStream(cur)), "md_append_paged_kv")
 
 
 def read_kv(k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, n_max=None, kv_scales=None, kv_layout="NHD"):
     """The inverse of update_kv, for every kind of cache: the last indptr[b + 1] - indptr[b] tokens of request b, as bf16, into rows indptr[b] ...
     of k and v [rows, KH, D] (in place; returns them).  Rows of positions in front of a request's first token or outside its pages stay as they
     were.  n_max: the most rows of a request (None: as many as there are rows)."""
-    _here("read_kv", k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen)
-    B = kv_page_indptr.numel() - 1
+    what = "read_kv"
+    cur = _here(what, k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen)
     page_size, KH, width = _kv_geom(kv_cache, kv_layout)
     D = k.shape[-1]
-    _checked_rows("read_kv", KH, D, k, v)
-    _checked_table("read_kv", B, indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
-    kv = _kv_args(kv_cache, kv_scales, kv_layout, D)
-    if not _is_mx(kv_cache) and width != D:
-        raise ValueError(f"read_kv: rows of {D} elements of a cache of {width}")
-    if B >= 1 and k.shape[0]:
-        check(_lib.load().md_read_paged_kv(_p(k), _p(v), k.stride(0), v.stride(0), _p(indptr), _p(kv_cache),
-                                           _pages(kv_page_indices, kv_page_indptr), _p(kv_page_indptr), _p(kv_page_lastlen), B, k.shape[0] if n_max is None else n_max, KH, D, page_size,
-                                           *kv, _stream()), "md_read_paged_kv")
+    kind, ks, vs = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    rows, B = _rows_of(what, k, KH, D), _table_of(what, indptr, kv_page_indices, kv_page_indptr, kv_page_lastlen)
+    if _rows_of(what, v, KH, D) != rows:
+        raise ValueError(f"{what}: {rows} rows of k and {v.shape[0]} of v")
+    if width != D and not _is_mx(kv_cache):
+        raise ValueError(f"{what}: rows of {D} elements of a cache of {width}")
+    if B >= 1 and rows:
+        check(_lib.load().md_read_paged_kv(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), indptr.data_ptr(), kv_cache.data_ptr(),
+                                           _pages(kv_page_indices, kv_page_indptr), kv_page_indptr.data_ptr(), kv_page_lastlen.data_ptr(), B,
+                                           rows if n_max is None else n_max, KH, D, page_size, kind, ks, vs,
+                                           torch._C._cuda_getCurrentRawStream(cur)), "md_read_paged_kv")
     return k, v
 
 
@@ -245,26 +272,13 @@ def rope_append(q, k, v, indptr, offsets, table: RopeTable, kv_cache, page_indic
                 kv_scales=None, kv_layout="NHD"):
     """Fused mylib::rope + mylib::update_kv (+ second cache for self-spec verify).  Returns rotated q.
     kv_cache may be fp8 (with kv_scales) and/or HND (kv_layout), or block-scaled (mx_kv_cache); kv_cache2 is always bf16 NHD."""
+    if _is_mx(kv_cache):
+        return _rope_append_mx(q, k, v, indptr, offsets, table, kv_cache, page_indices, page_indptr, last_page_len, kv_cache2, page_indices2,
+                               page_indptr2, last_page_len2, n_max, kv_scales, kv_layout)
     _gpu(q, k, v, kv_cache, kv_cache2)
     B = indptr.numel() - 1
     H, D = q.shape[1], q.shape[2]
     KH = k.shape[1]
-    if _is_mx(kv_cache):
-        _here("rope_append", q, k, v, indptr, offsets, table.table, kv_cache, page_indices, page_indptr, last_page_len, kv_cache2, page_indices2,
-              page_indptr2, last_page_len2)
-        _checked_rows("rope_append", H, D, q)
-        _checked_rows("rope_append", _kv_geom(kv_cache, kv_layout)[1], D, k, v)
-        _checked_table("rope_append", B, indptr, page_indices, page_indptr, last_page_len, offsets)
-        if q.shape[0] != k.shape[0] or table.head_dim != D:
-            raise ValueError("rope_append: as many rows of q as of k and a table of their head size expected")
-        if kv_cache2 is not None:
-            _checked_table("rope_append", B, indptr, page_indices2, page_indptr2, last_page_len2)
-            if (kv_cache2.dtype != torch.bfloat16 or not kv_cache2.is_contiguous()
-                    or kv_cache2.shape[1:] != (2, kv_cache.shape[3], KH, D)):
-                raise ValueError("rope_append: the second cache must be bfloat16 [pages, 2, page, KH, D] with the first one's page size")
-        if B < 1 or not q.shape[0]:
-            return torch.empty_like(q, memory_format=torch.contiguous_format)
-        page_indices = page_indices if page_indices.numel() else page_indptr
     if n_max is None:
         n_max = max((q.shape[0] + B - 1) // B, 1)
     q_out = torch.empty((q.shape[0], H, D), dtype=q.dtype, device=q.device)
@@ -273,7 +287,36 @@ def rope_append(q, k, v, indptr, offsets, table: RopeTable, kv_cache, page_indic
                              _p(_i32(indptr)), _p(_i32(offsets)), B, n_max, H, KH, D, _p(table.table), table.max_pos,
                              _p(kv_cache), _p(_i32(page_indices)), _p(_i32(page_indptr)), _p(_i32(last_page_len)),
                              _p(kv_cache2), _p(page_indices2), _p(page_indptr2), _p(last_page_len2),
-                             _kv_geom(kv_cache, kv_layout)[0], *_kv_args(kv_cache, kv_scales, kv_layout, D), _stream()),
+                             _kv_geom(kv_cache, kv_layout)[0], *_kv_args(kv_cache, kv_scales, kv_layout), _stream()),
+          "md_rope_append")
+    return q_out
+
+
+def _rope_append_mx(q, k, v, indptr, offsets, table, kv_cache, page_indices, page_indptr, last_page_len, kv_cache2, page_indices2, page_indptr2,
+                    last_page_len2, n_max, kv_scales, kv_layout):
+    what = "rope_append"
+    cur = _here(what, q, k, v, indptr, offsets, table.table, kv_cache, page_indices, page_indptr, last_page_len)
+    page_size, KH, _ = _kv_geom(kv_cache, kv_layout)
+    H, D = q.shape[1], q.shape[2]
+    kind, _, _ = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    rows, B = _rows_of(what, q, H, D), _table_of(what, indptr, page_indices, page_indptr, last_page_len, offsets)
+    if _rows_of(what, k, KH, D) != rows or _rows_of(what, v, KH, D) != rows or table.head_dim != D:
+        raise ValueError(f"{what}: as many rows of k and v as of q ({rows}) and a table of their head size ({D}) expected")
+    second = (None, None, None, None)
+    if kv_cache2 is not None:
+        _here(what, kv_cache2, page_indices2, page_indptr2, last_page_len2)
+        if _table_of(what, indptr, page_indices2, page_indptr2, last_page_len2) != B:
+            raise ValueError(f"{what}: page tables of {B} and {page_indptr2.numel() - 1} requests")
+        if kv_cache2.dtype is not torch.bfloat16 or not kv_cache2.is_contiguous() or kv_cache2.shape[1:] != (2, page_size, KH, D):
+            raise ValueError(f"{what}: the second cache must be contiguous bfloat16 [pages, 2, page, KH, D] with the first one's page size")
+        second = (kv_cache2.data_ptr(), _pages(page_indices2, page_indptr2), page_indptr2.data_ptr(), last_page_len2.data_ptr())
+    q_out = torch.empty((rows, H, D), dtype=q.dtype, device=q.device)
+    if B < 1 or not rows:
+        return q_out
+    check(_lib.load().md_rope_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), k.stride(0), v.stride(0), q_out.data_ptr(),
+                                     indptr.data_ptr(), offsets.data_ptr(), B, rows if n_max is None else n_max, H, KH, D, table.table.data_ptr(),
+                                     table.max_pos, kv_cache.data_ptr(), _pages(page_indices, page_indptr), page_indptr.data_ptr(),
+                                     last_page_len.data_ptr(), *second, page_size, kind, None, None, torch._C._cuda_getCurrentRawStream(cur)),
           "md_rope_append")
     return q_out
 
@@ -333,34 +376,37 @@ def paged_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _window_workspace(*shape):
+    return _lib.load().md_window_attn_workspace_bytes(*shape)
+
+
 def _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, n_max, max_pages_per_req, workspace, causal, sm_scale, out,
                       kv_scales, kv_layout, window, sinks):
     what = "paged_attention"
-    _here(what, q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, out)
-    B = page_indptr.numel() - 1
+    cur = _here(what, q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, out)
     page_size, KH, width = _kv_geom(kv_cache, kv_layout)
     _, H, D = q.shape
-    _checked_rows(what, H, D, q)
-    _checked_table(what, B, qo_indptr, page_indices, page_indptr, last_page_len)
-    kv = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    kind, ks, vs = _kv_args(kv_cache, kv_scales, kv_layout, D)
+    rows, B = _rows_of(what, q, H, D), _table_of(what, qo_indptr, page_indices, page_indptr, last_page_len)
     if not causal:
         raise ValueError(f"{what}: attention with a window or over a block-scaled cache is causal")
-    if H % KH or (not _is_mx(kv_cache) and width != D):
+    if H % KH or (width != D and not _is_mx(kv_cache)):
         raise ValueError(f"{what}: {H} query heads of {D} over {KH} kv heads of {width}")
     if (window is not None and window < 1) or sinks < 0:
         raise ValueError(f"{what}: window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        out = torch.empty((rows, H, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
         raise ValueError(f"{what}: out must be a contiguous tensor like q")
-    if B < 1 or not q.shape[0]:
+    if B < 1 or not rows:
         return out
     window, sinks = 0 if window is None else min(window, 1 << 30), min(sinks, 1 << 30)
-    lib = _lib.load()
-    ws = workspace.get(lib.md_window_attn_workspace_bytes(B, n_max, H, KH, D, max_pages_per_req, page_size, kv[0], window, sinks))
-    check(lib.md_window_attn(_p(q), q.stride(0), _p(kv_cache), _p(out), _p(qo_indptr), _pages(page_indices, page_indptr), _p(page_indptr), _p(last_page_len), B,
-                             n_max, H, KH, D, page_size, window, sinks, float(1.0 / math.sqrt(D) if sm_scale is None else sm_scale),
-                             max_pages_per_req, *kv, _p(ws), ws.numel(), _stream()), "md_window_attn")
+    ws = workspace.get(_window_workspace(B, n_max, H, KH, D, max_pages_per_req, page_size, kind, window, sinks))
+    check(_lib.load().md_window_attn(q.data_ptr(), q.stride(0), kv_cache.data_ptr(), out.data_ptr(), qo_indptr.data_ptr(),
+                                     _pages(page_indices, page_indptr), page_indptr.data_ptr(), last_page_len.data_ptr(), B, n_max, H, KH, D,
+                                     page_size, window, sinks, 1.0 / math.sqrt(D) if sm_scale is None else sm_scale, max_pages_per_req, kind, ks,
+                                     vs, ws.data_ptr(), ws.numel(), torch._C._cuda_getCurrentRawStream(cur)), "md_window_attn")
     return out
 
 
