@@ -49,6 +49,20 @@ __device__ __forceinline__ unsigned infinite_halves(unsigned u, bool negative) {
     return m & 0x3f803f80u;
 }
 
+// Weights are exp2(score * factor - reference) in one operation, whose exponent is off by at most 2^-24 of the reference; beyond 2^12 scores are
+// rounded in front of it, so that the largest one's weight is 1 however large it is.
+template <int N>
+__device__ __forceinline__ float exponent_factor(float m, float factor, float (&v)[N]) {
+    if (__builtin_amdgcn_ballot_w64(fabsf(m) > 4096.f && m != kLowest) == 0) return factor;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        float x = v[e] * factor;
+        asm volatile("" : "+v"(x));          // a branch of the wavefront, not a select
+        v[e] = x;
+    }
+    return 1.0f;
+}
+
 // Tiles of KT keys that rows between the positions lo and hi look at: those of the first tokens, then those from the lowest window on
 struct Tiles {
     int first, w0, count;       // tiles of the first tokens, the window's first tile, tiles in all

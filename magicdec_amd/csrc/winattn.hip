@@ -22,29 +22,31 @@
 
 namespace {
 
-template <int D, int QT>
+template <int D, int QT, int KG>
 __host__ __device__ constexpr int win_wave_lds() {
-    const int image = (D / 16) * kVSub, merge = QT * D * 64 + QT * 128;
+    const int image = KG * (D / 16) * kVSub, merge = QT * D * 64 + QT * 128;
     return ((image > merge ? image : merge) + 255) / 256 * 256;
 }
 
 constexpr int kWaves = 4;
 
-template <int D, int QT, int KIND>
+// KG: groups of 32 keys in a tile
+template <int D, int QT, int KIND, int KG>
 __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinParams p) {
+    constexpr int KT = KG * 32, VG = (D / 16) * kVSub;
     constexpr int EB = kv_element_bytes(KIND, D);        // bytes of a row's elements
     constexpr bool MX = kv_is_mx(KIND);
     constexpr int KS = D / 32, NB = D / 16, SB = D / 32;  // matrix steps of a score, 16-d blocks, scales of a row
     // keys: a lane's loads of a row, their dwords, elements and matrix steps
     constexpr int KI = EB >= 64 ? EB / 64 : 1, KW = EB >= 64 ? 4 : EB / 16, EL = D / (4 * KI), SPL = EL / 8;
-    // values: 16-byte pieces of a row, rows of a load, loads
+    // values: 16-byte pieces of a row, rows of a load, loads of a group
     constexpr int CH = EB / 16, RPI = 64 / CH, NL = 32 / RPI;
     // 8 neighbouring lanes write 16-byte halves of 32-byte rows: the upper half of the pieces begin with their second half, so that they
     // lie in different banks; in the d blocks from 4 on the halves are then the other way round (undone where rows are stored)
     constexpr bool SWAP = KIND != MD_KV_BF16 && D == 128;
-    constexpr int WAVE_LDS = win_wave_lds<D, QT>();
-    // tiles in flight: with two row tiles of 128 a second one spills (mxfp8, 64 requests of 8 100 keys, 20 rows a kv head: 223 us, 198 with one)
-    constexpr int NS = QT == 2 && D == 128 && KIND != MD_KV_MXFP4 ? 1 : 2;
+    constexpr int WAVE_LDS = win_wave_lds<D, QT, KG>();
+    // tiles in flight: as many as the registers hold
+    constexpr int NS = KG * EB * QT > 256 || (QT == 2 && D == 128 && KIND != MD_KV_MXFP4) ? 1 : 2;
 
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     const int tid = threadIdx.x;
@@ -84,22 +86,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     hi = __builtin_amdgcn_readfirstlane(hi);
     lo = __builtin_amdgcn_readfirstlane(lo);
     const int hi_low = p.window > 0 ? hi - p.window : -1;
-    const Tiles tiles(lo, min(hi + 1, kv_len), p.window, p.sinks, 32);
+    const Tiles tiles(lo, min(hi + 1, kv_len), p.window, p.sinks, KT);
     const int per = (tiles.count + p.nsplit - 1) / p.nsplit;
     const int t_begin = split * per, t_end = min(tiles.count, t_begin + per);
 
-    bf16x8 qf[QT][KS];
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const int R = (qg * QT + qt) * 16 + lq;
-        const int i = R / g, r = R - i * g;
-        const bf16_t* qp = p.q + (int64_t)(q0 + i) * p.q_row_stride + (kvh * g + r) * D;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-            qf[qt][s] = R < nrows ? *reinterpret_cast<const bf16x8*>(qp + (s / SPL) * 4 * EL + lc * EL + (s % SPL) * 8) : z;
-        }
-    }
     const float sl2 = KIND == MD_KV_FP8_E4M3 ? p.scale_log2 * p.k_scale[kvh] : p.scale_log2;
     const float vsc = KIND == MD_KV_FP8_E4M3 ? p.v_scale[kvh] : 1.0f;
     f32x4 o[QT][NB];
@@ -115,25 +105,25 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     unsigned char* image = smem + wave * WAVE_LDS;
     const int wrow = lane / CH, wch = lane % CH;
     const bool swp = SWAP && wch >= CH / 2;
-    const int vra = (lc * 4 + (lq >> 2)) * 32 + (lq & 3) * 8;       // + nb * kVSub, + 512 for the second 16 keys
+    const int vra = (lc * 4 + (lq >> 2)) * 32 + (lq & 3) * 8;       // + kg * VG + nb * kVSub, + 512 for the second 16 keys
 
     struct Staged {
-        unsigned k[2][KI * KW];
-        u32x4 v[NL];
-        unsigned scale;
+        unsigned k[2 * KG][KI * KW];
+        u32x4 v[KG][NL];
+        unsigned scale[KG];
     };
     Staged st[NS];
     const unsigned koff = (unsigned)(lq * p.g.slot + lc * KW * 4), voff = (unsigned)(wrow * p.g.slot + wch * 16);
     const int64_t soff = (lane >= 32 ? p.g.half : 0) + (lane & 31) * SB;
     PageCursor at(p, pg0, room);
     auto tile_base = [&](int i) {
-        at.seek(tiles.at(i) * 32);
+        at.seek(tiles.at(i) * KT);
         return p.cache + at.id() * p.g.page + (int64_t)kvh * p.g.head + (int64_t)at.slot * p.g.slot;
     };
-    auto issue = [&](int i, Staged& s) {
+    auto issue = [&](int i, Staged& s) __attribute__((always_inline)) {
         const unsigned char* base = tile_base(i);
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2 * KG; ++kb)
 #pragma unroll
             for (int k = 0; k < KI; ++k) {
                 const unsigned char* from = base + (int64_t)kb * 16 * p.g.slot + koff + k * 64;
@@ -148,12 +138,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
                 }
             }
         if constexpr (MX) {
-            const unsigned char* from = base - (int64_t)at.slot * (EB - SB) + p.g.scales + soff;
-            s.scale = SB == 4 ? *reinterpret_cast<const unsigned*>(from) : *reinterpret_cast<const unsigned short*>(from);
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg) {
+                const unsigned char* from = base - (int64_t)at.slot * (EB - SB) + p.g.scales + kg * 32 * SB + soff;
+                s.scale[kg] = SB == 4 ? *reinterpret_cast<const unsigned*>(from) : *reinterpret_cast<const unsigned short*>(from);
+            }
         }
 #pragma unroll
-        for (int j = 0; j < NL; ++j)
-            s.v[j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)j * RPI * p.g.slot + voff));
+        for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+            for (int j = 0; j < NL; ++j)
+                s.v[kg][j] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)(kg * 32 + j * RPI) * p.g.slot + voff));
     };
     auto scale_of = [&](unsigned scales, int row, int block) {       // row 0..31 keys, 32..63 values
         const unsigned u = (unsigned)__builtin_amdgcn_ds_bpermute(row * 4, (int)scales);
@@ -178,98 +173,103 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
             for (int w = 0; w < 4; ++w) mx8_to_bf16(x[w], scale, y[2 * w], y[2 * w + 1]);
         }
     };
-    auto put_values = [&](int j, const unsigned (&y)[VD]) {
-        const int row = (wrow + j * RPI) * 32;
+    auto put_values = [&](int kg, int j, const unsigned (&y)[VD]) {
+        unsigned char* row = image + kg * VG + (wrow + j * RPI) * 32;
         if constexpr (KIND == MD_KV_BF16) {
-            *reinterpret_cast<u32x4*>(image + (wch >> 1) * kVSub + row + (wch & 1) * 16) = u32x4{y[0], y[1], y[2], y[3]};
+            *reinterpret_cast<u32x4*>(row + (wch >> 1) * kVSub + (wch & 1) * 16) = u32x4{y[0], y[1], y[2], y[3]};
         } else {
             constexpr int SUBS = VD / 8;
 #pragma unroll
             for (int s = 0; s < SUBS; ++s) {
-                unsigned char* at = image + (wch * SUBS + s) * kVSub + row;
-                *reinterpret_cast<u32x4*>(at + (swp ? 16 : 0)) = u32x4{y[8 * s], y[8 * s + 1], y[8 * s + 2], y[8 * s + 3]};
-                *reinterpret_cast<u32x4*>(at + (swp ? 0 : 16)) = u32x4{y[8 * s + 4], y[8 * s + 5], y[8 * s + 6], y[8 * s + 7]};
+                unsigned char* to = row + (wch * SUBS + s) * kVSub;
+                *reinterpret_cast<u32x4*>(to + (swp ? 16 : 0)) = u32x4{y[8 * s], y[8 * s + 1], y[8 * s + 2], y[8 * s + 3]};
+                *reinterpret_cast<u32x4*>(to + (swp ? 0 : 16)) = u32x4{y[8 * s + 4], y[8 * s + 5], y[8 * s + 6], y[8 * s + 7]};
             }
         }
     };
-    auto value_scale = [&](unsigned scales, int j) {
-        return MX ? scale_of(scales, 32 + wrow + j * RPI, KIND == MD_KV_MXFP4 ? wch : wch >> 1) : 1.0f;
-    };
+    constexpr int VB = KIND == MD_KV_MXFP4 ? 32 : 16;                // elements of a lane's 16 bytes
     // one wavefront's LDS operations run in order: the compiler has to keep them so, too
     auto in_order = [&] {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
-    auto value_fragment = [&](int nb) {
-        const bf16x4 a = lds_read_tr(image + nb * kVSub + vra), c = lds_read_tr(image + nb * kVSub + 512 + vra);
+    auto value_fragment = [&](int kg, int nb) {
+        const unsigned char* from = image + kg * VG + nb * kVSub + vra;
+        const bf16x4 a = lds_read_tr(from), c = lds_read_tr(from + 512);
         return __builtin_shufflevector(a, c, 0, 1, 2, 3, 4, 5, 6, 7);
     };
     // infinite values and NaN of tile i go to the rows that see them
-    auto spread = [&](int i, const unsigned (&hidden)[QT]) {
+    auto spread = [&](int i, const unsigned (&hidden)[QT]) __attribute__((always_inline)) {
         const unsigned char* base = tile_base(i);
 #pragma unroll 1
         for (int negative = 0; negative < 2; ++negative) {
             in_order();
 #pragma unroll
-            for (int j = 0; j < NL; ++j) {
-                const int row = wrow + j * RPI;
-                const u32x4 x = *reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)j * RPI * p.g.slot + voff);
-                float scale = 1.0f;
-                if constexpr (MX)
-                    scale = mx_scale(base[p.g.half - (int64_t)at.slot * (EB - SB) + p.g.scales + row * SB + (KIND == MD_KV_MXFP4 ? wch : wch >> 1)]);
-                unsigned y[VD];
-                values(x, scale, y);
+            for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
-                for (int e = 0; e < VD; ++e) y[e] = infinite_halves(y[e], negative != 0);
-                put_values(j, y);
-            }
+                for (int j = 0; j < NL; ++j) {
+                    const int row = kg * 32 + wrow + j * RPI;
+                    const u32x4 x = *reinterpret_cast<const u32x4*>(base + p.g.half + (int64_t)(kg * 32 + j * RPI) * p.g.slot + voff);
+                    float scale = 1.0f;
+                    if constexpr (MX) scale = mx_scale(base[p.g.half - (int64_t)at.slot * (EB - SB) + p.g.scales + row * SB + wch * VB / 32]);
+                    unsigned y[VD];
+                    values(x, scale, y);
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) y[e] = infinite_halves(y[e], negative != 0);
+                    put_values(kg, j, y);
+                }
             in_order();
             const float add = negative ? -INFINITY : INFINITY;
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) {
-                bf16x8 seen;
+            for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) seen[e] = hidden[qt] >> e & 1 ? (bf16_t)0.f : (bf16_t)1.f;
+                for (int kg = 0; kg < KG; ++kg) {
+                    bf16x8 seen;
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_fragment(nb), seen, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    for (int e = 0; e < 8; ++e) seen[e] = hidden[qt] >> (kg * 8 + e) & 1 ? (bf16_t)0.f : (bf16_t)1.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n[r] > 0.f) o[qt][nb][r] += add;
+                    for (int nb = 0; nb < NB; ++nb) {
+                        const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value_fragment(kg, nb), seen, f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (n[r] > 0.f) o[qt][nb][r] += add;
+                    }
                 }
-            }
         }
         in_order();
     };
 
-    auto process = [&](auto more, int i, Staged& s) {
+    bf16x8 qf[QT][KS];
+    auto process = [&](auto more, int i, Staged& s) __attribute__((always_inline)) {
         const int t = tiles.at(i);
-        const bool need_mask = t * 32 + 31 > lo || (t * 32 <= hi_low && t * 32 + 31 >= p.sinks);
+        const bool need_mask = t * KT + KT - 1 > lo || (t * KT <= hi_low && t * KT + KT - 1 >= p.sinks);
         bool infinite = false;
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-            unsigned y[VD];
-            values(s.v[j], value_scale(s.scale, j), y);
-            if (need_mask) {
+        for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
-                for (int e = 0; e < VD; ++e) {
-                    const unsigned n = nonfinite_halves(y[e]);
-                    infinite |= n != 0;
-                    y[e] &= ~n;
+            for (int j = 0; j < NL; ++j) {
+                unsigned y[VD];
+                values(s.v[kg][j], MX ? scale_of(s.scale[kg], 32 + wrow + j * RPI, wch * VB / 32) : 1.0f, y);
+                if (need_mask) {
+#pragma unroll
+                    for (int e = 0; e < VD; ++e) {
+                        const unsigned n = nonfinite_halves(y[e]);
+                        infinite |= n != 0;
+                        y[e] &= ~n;
+                    }
                 }
+                put_values(kg, j, y);
             }
-            put_values(j, y);
-        }
-        f32x4 sc[QT][2];
+        f32x4 sc[QT][2 * KG];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < 2 * KG; ++kb) {
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) sc[qt][kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < KI; ++k) {
                 // a lane's piece of a row is one block's, or a half of it
-                const float scale = MX ? scale_of(s.scale, kb * 16 + lq, EL == 32 ? lc : k * 2 + (lc >> 1)) : 1.0f;
+                const float scale = MX ? scale_of(s.scale[kb / 2], (kb & 1) * 16 + lq, EL == 32 ? lc : k * 2 + (lc >> 1)) : 1.0f;
 #pragma unroll
                 for (int h = 0; h < SPL; ++h) {
                     unsigned y[4];
@@ -296,19 +296,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
         }
         in_order();
 
-        bf16x8 pf[QT];
+        bf16x8 pf[QT][KG];
         unsigned hidden[QT];
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
-            float v[8];
+            float v[8 * KG];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = sc[qt][e >> 2][e & 3] * sl2;     // rounded here: the largest minus the reference is 0
+            for (int e = 0; e < 8 * KG; ++e) v[e] = sc[qt][e >> 2][e & 3];
             hidden[qt] = 0;
             if (need_mask) {
                 // a branch of the wavefront: volatile, or every tile would compare and select
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int pos = t * 32 + (e >> 2) * 16 + lc * 4 + (e & 3);
+                for (int e = 0; e < 8 * KG; ++e) {
+                    const int pos = t * KT + (e >> 2) * 16 + lc * 4 + (e & 3);
                     const bool out = pos > lim[qt] || (pos <= low[qt] && pos >= p.sinks);
                     float x = out ? -INFINITY : v[e];
                     asm volatile("" : "+v"(x));
@@ -318,8 +318,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
             }
             float mx = v[0];
 #pragma unroll
-            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, v[e]);
-            mx = max_over_32(max_over_16(mx));
+            for (int e = 1; e < 8 * KG; ++e) mx = fmaxf(mx, v[e]);
+            mx = max_over_32(max_over_16(mx)) * sl2;
             if (__builtin_amdgcn_ballot_w64(mx > m[qt]) != 0) {         // some row has a new reference
                 const float mnew = fmaxf(m[qt], mx), alpha = __builtin_amdgcn_exp2f(m[qt] - mnew);
                 m[qt] = mnew;
@@ -327,32 +327,50 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) o[qt][nb] *= alpha;
             }
+            const float times = exponent_factor(m[qt], sl2, v);
             float ps = 0.f;
-            f32x8 w;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                w[e] = __builtin_amdgcn_exp2f(v[e] - m[qt]);
-                ps += w[e];
+            for (int kg = 0; kg < KG; ++kg) {
+                f32x8 w;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    w[e] = __builtin_amdgcn_exp2f(fmaf(v[kg * 8 + e], times, -m[qt]));
+                    ps += w[e];
+                }
+                pf[qt][kg] = __builtin_convertvector(w, bf16x8);       // the matrix instruction's operand: weights from 0 to 1, off by 2^-8 of themselves
             }
             l[qt] += ps;
-            pf[qt] = __builtin_convertvector(w, bf16x8);       // the matrix instruction's operand: weights from 0 to 1, off by 2^-9 of themselves
         }
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            const bf16x8 vf = value_fragment(nb);
+        for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) o[qt][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qt], o[qt][nb], 0, 0, 0);
-        }
+            for (int nb = 0; nb < NB; ++nb) {
+                const bf16x8 vf = value_fragment(kg, nb);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) o[qt][nb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[qt][kg], o[qt][nb], 0, 0, 0);
+            }
         if (need_mask && __builtin_amdgcn_ballot_w64(infinite) != 0) spread(i, hidden);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
 
-    // steady state: loads of the tile NS turns on are issued without a condition, so that waits are for the tile at hand alone
     int i = t_begin + wave;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
         if (i + s * kWaves < t_end) issue(i + s * kWaves, st[s]);
+    // the queries behind the first tiles' loads
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int R = (qg * QT + qt) * 16 + lq;
+        const int qi = R / g, r = R - qi * g;
+        const bf16_t* qp = p.q + (int64_t)(q0 + qi) * p.q_row_stride + (kvh * g + r) * D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            qf[qt][s] = R < nrows ? *reinterpret_cast<const bf16x8*>(qp + (s / SPL) * 4 * EL + lc * EL + (s % SPL) * 8) : z;
+        }
+    }
+    // steady state: loads of the tile NS turns on are issued without a condition, so that waits are for the tile at hand alone
     for (; i + (2 * NS - 1) * kWaves < t_end; i += NS * kWaves) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) process(std::true_type{}, i + s * kWaves, st[s]);
@@ -400,8 +418,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
             acc += ow[(qt * D + d) * 16 + qq] * a;
         }
         if (p.nsplit == 1) {
-            const int i = R / g;
-            p.out[((int64_t)(q0 + i) * p.H + kvh * g + R - i * g) * D + d] = f32_to_bf16(L == 0.f ? 0.f : acc * (vsc / L));
+            const int qi = R / g;
+            p.out[((int64_t)(q0 + qi) * p.H + kvh * g + R - qi * g) * D + d] = f32_to_bf16(L == 0.f ? 0.f : acc * (vsc / L));
         } else {
             const int64_t slot = (((int64_t)pair * p.n_qgroups + qg) * p.nsplit + split) * ROWS + Rl;
             p.ws_o[slot * D + d] = acc;
@@ -432,13 +450,30 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinParams p, in
     float M = kLowest, L = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     if (live) {
-        for (int s = sg; s < p.nsplit; s += SG) {
-            const int64_t slot = ((int64_t)item * p.nsplit + s) * rows + Rl;
-            const float ms = p.ws_ml[slot * 2], mn = fmaxf(M, ms);
-            const float a = __builtin_amdgcn_exp2f(M - mn), c = __builtin_amdgcn_exp2f(ms - mn);
-            const f32x4 os = *reinterpret_cast<const f32x4*>(p.ws_o + slot * D + v * 4);
-            L = L * a + p.ws_ml[slot * 2 + 1] * c;
-            acc = acc * a + os * c;
+        for (int s0 = sg; s0 < p.nsplit; s0 += 8 * SG) {           // eight requested together: one wait
+            float ms[8], ls[8];
+            f32x4 os[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int s = s0 + u * SG;
+                const int64_t slot = ((int64_t)item * p.nsplit + (s < p.nsplit ? s : s0)) * rows + Rl;
+                ms[u] = p.ws_ml[slot * 2];
+                ls[u] = p.ws_ml[slot * 2 + 1];
+                os[u] = *reinterpret_cast<const f32x4*>(p.ws_o + slot * D + v * 4);
+            }
+            float mn = M;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) mn = fmaxf(mn, ms[u]);
+            const float a = __builtin_amdgcn_exp2f(M - mn);
+            L *= a;
+            acc *= a;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (s0 + u * SG < p.nsplit) {
+                    const float c = __builtin_amdgcn_exp2f(ms[u] - mn);
+                    L += ls[u] * c;
+                    acc += os[u] * c;
+                }
             M = mn;
         }
     }
@@ -471,30 +506,64 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinParams p, in
 // How a call's rows and keys lie over workgroups
 struct WinPlan {
     int nw;                 // wavefronts of a workgroup of winprompt.hip, 0: the kernel above
+    int kg;                 // groups of 32 keys in its tiles
     int rows, n_qgroups, nsplit;
     size_t slots;
 };
 
-WinPlan window_plan(int B, int n_max, int H, int KH, int max_pages, int page_size, int window, int sinks) {
+// All in us, 8 kv heads unless said.
+WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int page_size, int kind, int window, int sinks) {
     WinPlan pl;
-    const int64_t rows = (int64_t)n_max * (H / KH);
-    pl.nw = rows <= 32 ? 0 : rows >= 256 ? 8 : 4;
+    const int64_t rows = (int64_t)n_max * (H / KH), pairs = (int64_t)B * KH;
+    // keys that one row looks at, and those that neighbouring ones do besides, at most
+    const int64_t all = (int64_t)max_pages * page_size;
+    const auto seen = [&](int64_t n) { return window > 0 ? std::min<int64_t>(all, (int64_t)window + n + std::min<int64_t>(sinks, all)) : all; };
+    const auto groups = [&](int64_t n) { return pairs * ((rows + n - 1) / n); };
+    // More than 32 rows: in workgroups of 8 wavefronts where those are many or walk far (512 x 4 heads over 4 000 keys of 128 in bf16: 60 in
+    // workgroups of 4, 54 of 8; over 700 keys 27 and 31), or where one of them, of larger tiles, does what one of 4 did (16 x 32 x 4 over 600 22,
+    // 28 of 4).  In groups of 32 on the kernel above, which shares a group's keys over its wavefronts, where these fill the chip by themselves and
+    // walk a short way: 16 requests x 10 x 4 heads over 600 keys 20, 24 in workgroups of 4; 512 x 4 of 64 over 700 17, 21; but 4 x 128 x 4 of 128
+    // over 600 in bf16 30, 26
+    const int64_t of32 = groups(32), walk = groups(256) * seen(n_max);
+    const bool short_way = seen(rows) <= 768 && of32 >= 200 && of32 <= 512 && (D == 64 || rows <= 64);
+    pl.nw = rows <= 32 || short_way ? 0 : rows >= 256 ? (walk >= 100000 ? 8 : 4) : rows > 96 && rows <= 128 && D == 128 && walk < 100000 ? 8 : 4;
     pl.rows = pl.nw ? pl.nw * 32 : rows <= 16 ? 16 : 32;
     pl.n_qgroups = (int)((rows + pl.rows - 1) / pl.rows);
-    // keys that a row group looks at, at most
-    int64_t keys = (int64_t)max_pages * page_size;
-    if (window > 0) keys = std::min<int64_t>(keys, (int64_t)window + pl.rows + std::min<int64_t>(sinks, keys));
-    const int64_t groups = (int64_t)B * KH * pl.n_qgroups;
-    pl.nsplit = pl.nw ? (int)std::max<int64_t>(1, std::min<int64_t>({256 / groups, keys / 384, 32}))
-                      : (int)std::max<int64_t>(1, std::min<int64_t>({512 / groups, keys / 256, 64}));
-    pl.slots = pl.nsplit > 1 ? (size_t)groups * pl.nsplit * pl.rows : 0;
+    const int64_t keys = seen(std::min<int64_t>(n_max, (pl.rows + H / KH - 1) / (H / KH) + 1)), have = pairs * pl.n_qgroups;
+    // Keys over several workgroups, of enough keys each to pay for the launch that joins them (3.5).
+    int64_t want, most;
+    if (pl.nw) {
+        // one a CU, or what it holds of them where there are many: 4 x 10 x 4 rows over 4 000 keys 27 in 256, 29 in 512; 16 x 10 x 4 78 in 256, 57 in 512
+        const bool many = have >= 96;
+        want = (!many || pl.nw == 8 ? 256 : D == 64 ? 1024 : 512) / have, most = many ? keys / 1024 + 1 : pl.nw == 8 ? (keys + 255) / 256 : (keys + 159) / 160;
+    } else if (rows > 32) {
+        want = most = 1;
+    } else {
+        // One a CU up to half as many (4 x 4 rows over 5 000 keys in bf16: 70 whole, 22 in 256, 25 in 512), two where 8- or 4-bit streams stay long
+        // (8 x 4 over 8 000 37 and 34); beyond that three where streams are long (32 x 4 over 9 000 120 whole, 110), and so where the last
+        // workgroups would leave CUs behind (40 x 4 over 9 000 in bf16 311 whole, 242 in three; 48 x 4 337 and 289 in two)
+        const int64_t stream = keys * 2 * kv_row_bytes(kind, D);
+        const bool long_way = stream >= 700000, left = have * 100 < (have + 511) / 512 * 512 * 85;
+        if (have <= 128)
+            want = (kind != MD_KV_BF16 && keys * have >= 512000 ? 512 : 256) / have;
+        else if (have <= 256)
+            want = kind != MD_KV_BF16 && long_way ? 768 / have : 1;
+        else
+            want = !long_way || !left ? 1 : have <= 352 ? 3 : 2;
+        most = keys <= 512 ? 1 : keys / 128;
+    }
+    pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, pl.nw ? 32 : 64}));
+    // 64 keys at a time where that spills nothing and the stream is long: 4-bit heads of 64, 64 requests of 16 036 keys x 16 rows 133 -> 114, of 1 000 12.9
+    // -> 12.2; one request of 1 500 in eight parts 8.5 -> 9.9
+    pl.kg = kind == MD_KV_MXFP4 && D == 64 && pl.rows == 16 && page_size % 64 == 0 && keys / pl.nsplit >= 1024 ? 2 : 1;
+    pl.slots = pl.nsplit > 1 ? (size_t)have * pl.nsplit * pl.rows : 0;
     return pl;
 }
 
-template <int D, int QT, int KIND>
+template <int D, int QT, int KIND, int KG>
 int launch_window(const WinParams& p, int grid, hipStream_t st) {
-    constexpr int lds = kWaves * win_wave_lds<D, QT>();
-    auto k = window_attn_kernel<D, QT, KIND>;
+    constexpr int lds = kWaves * win_wave_lds<D, QT, KG>();
+    auto k = window_attn_kernel<D, QT, KIND, KG>;
     if constexpr (lds > 64 * 1024) {
         static MdPerDeviceOnce once;
         if (once.first()) {
@@ -512,17 +581,19 @@ int launch_window(const WinParams& p, int grid, hipStream_t st) {
 }
 
 template <int D, int KIND>
-int launch_window_rows(const WinParams& p, int rows, int grid, hipStream_t st) {
-    return rows == 16 ? launch_window<D, 1, KIND>(p, grid, st) : launch_window<D, 2, KIND>(p, grid, st);
+int launch_window_rows(const WinParams& p, const WinPlan& pl, int grid, hipStream_t st) {
+    if constexpr (D == 64 && KIND == MD_KV_MXFP4)
+        if (pl.kg == 2) return launch_window<D, 1, KIND, 2>(p, grid, st);
+    return pl.rows == 16 ? launch_window<D, 1, KIND, 1>(p, grid, st) : launch_window<D, 2, KIND, 1>(p, grid, st);
 }
 
 template <int D>
-int launch_window_kind(const WinParams& p, int kind, int rows, int grid, hipStream_t st) {
+int launch_window_kind(const WinParams& p, int kind, const WinPlan& pl, int grid, hipStream_t st) {
     switch (kind) {
-        case MD_KV_BF16: return launch_window_rows<D, MD_KV_BF16>(p, rows, grid, st);
-        case MD_KV_FP8_E4M3: return launch_window_rows<D, MD_KV_FP8_E4M3>(p, rows, grid, st);
-        case MD_KV_MXFP8: return launch_window_rows<D, MD_KV_MXFP8>(p, rows, grid, st);
-        default: return launch_window_rows<D, MD_KV_MXFP4>(p, rows, grid, st);
+        case MD_KV_BF16: return launch_window_rows<D, MD_KV_BF16>(p, pl, grid, st);
+        case MD_KV_FP8_E4M3: return launch_window_rows<D, MD_KV_FP8_E4M3>(p, pl, grid, st);
+        case MD_KV_MXFP8: return launch_window_rows<D, MD_KV_MXFP8>(p, pl, grid, st);
+        default: return launch_window_rows<D, MD_KV_MXFP4>(p, pl, grid, st);
     }
 }
 
@@ -538,7 +609,7 @@ int launch_window_prompt(const WinParams& p, int kind, int D, int nw, int grid, 
 template <int D>
 void launch_window_merge(const WinParams& p, int rows, hipStream_t st) {
     const int64_t threads = (int64_t)p.B * p.KH * p.n_qgroups * rows * (D / 4);
-    const int sg = p.nsplit <= 4 ? 1 : 8;
+    const int sg = p.nsplit <= 8 ? 1 : 8;
     const dim3 grid((unsigned)((threads * sg + 255) / 256));
     if (sg == 1)
         hipLaunchKernelGGL((window_merge_kernel<D, 1>), grid, dim3(256), 0, st, p, rows);
@@ -555,9 +626,8 @@ bool window_shape_ok(int B, int n_max, int H, int KH, int max_pages, int page_si
 
 extern "C" size_t md_window_attn_workspace_bytes(int B, int n_max, int H, int KH, int D, int max_pages_per_req, int page_size, int kv_dtype,
                                                  int window, int sinks) {
-    (void)kv_dtype;
     if (!window_shape_ok(B, n_max, H, KH, max_pages_per_req, page_size) || window < 0 || sinks < 0) return 0;
-    return window_plan(B, n_max, H, KH, max_pages_per_req, page_size, window, sinks).slots * ((size_t)D * 4 + 8) + 256;
+    return window_plan(B, n_max, H, KH, D, max_pages_per_req, page_size, kv_dtype & MD_KV_DTYPE_MASK, window, sinks).slots * ((size_t)D * 4 + 8) + 256;
 }
 
 extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* cache, void* out, const int32_t* qo_indptr,
@@ -583,7 +653,7 @@ extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* c
                  "md_window_attn: kv_dtype must be MD_KV_BF16, MD_KV_FP8_E4M3 (with per-head scales), MD_KV_MXFP8 or MD_KV_MXFP4");
     MD_CHECK_ARG(hnd || !kv_is_mx(kind), "md_window_attn: block-scaled pages are HND");
 
-    const WinPlan pl = window_plan(B, n_max, H, KH, max_pages_per_req, page_size, window, sinks);
+    const WinPlan pl = window_plan(B, n_max, H, KH, D, max_pages_per_req, page_size, kind, window, sinks);
     const size_t need = pl.slots * ((size_t)D * 4 + 8);
     if (pl.nsplit > 1 && !(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0)) {
         md_set_error("md_window_attn: workspace too small or misaligned (%zu < %zu)", workspace_bytes, need);
@@ -617,7 +687,7 @@ extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* c
     p.v_scale = kind == MD_KV_FP8_E4M3 ? v_scale : nullptr;
     hipStream_t st = (hipStream_t)stream;
     const int rc = pl.nw ? launch_window_prompt(p, kind, D, pl.nw, (int)grid, st)
-                   : D == 128 ? launch_window_kind<128>(p, kind, pl.rows, (int)grid, st) : launch_window_kind<64>(p, kind, pl.rows, (int)grid, st);
+                   : D == 128 ? launch_window_kind<128>(p, kind, pl, (int)grid, st) : launch_window_kind<64>(p, kind, pl, (int)grid, st);
     if (rc != MD_OK) return rc;
     if (pl.nsplit > 1) {
         D == 128 ? launch_window_merge<128>(p, pl.rows, st) : launch_window_merge<64>(p, pl.rows, st);

@@ -193,7 +193,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     };
     auto hidden = [&](int pos) { return pos > lim || (pos <= low && pos >= p.sinks); };
 
-    auto compute = [&](int i, const unsigned char* img) {
+    auto compute = [&](int i, const unsigned char* img) __attribute__((always_inline)) {
         const int pos0 = tiles.at(i) * KT;
         f32x16 sc[KG];
 #pragma unroll
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
                     o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value_fragment(img, kg, s16, db), pf[kg][s16], o[db], 0, 0, 0);
     };
     // infinite values and NaN of a tile to the rows that see them: by images of their signs in the values' place
-    auto spread = [&](int i, unsigned char* img) {
+    auto spread = [&](int i, unsigned char* img) __attribute__((always_inline)) {
         const int pos0 = tiles.at(i) * KT;
         const unsigned char* head = tile_base(pos0) + p.g.half;
         const int slot0 = at.slot;
