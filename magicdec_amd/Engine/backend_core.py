@@ -404,7 +404,8 @@ class SnapKVTargetBackend(_BackendBase):
         """num_pages: pages of the pool that `step` serves unequal sequences from, when it is not to be a whole page list per
         request (encode / inference are then unavailable).
         kv_dtype="fp8": the full-context cache is OCP e4m3fn with static per-head scales calibrated on the
-        first prefill chunk (not in the reference).  The compressed draft cache stays bf16.
+        first prefill chunk (not in the reference).  The compressed draft cache stays bf16.  "mxfp8" / "mxfp4": 8- or 4-bit elements with a
+        power-of-two scale for each 32 of a row, found as it is written; HND only.
         kv_layout="HND": the full-context cache keeps the rows of one kv head contiguous inside a page (the
         reference's flashinfer wrappers are planned "NHD": Engine/SnapKV/backend.py:30); same results, longer
         contiguous runs for the verify step's stream (matters for fp8 rows of 128 bytes).  None = default_kv_layout()."""

@@ -135,7 +135,9 @@ transformer_configs = {
 
 SINK = 16          # StreamingLLM sink tokens (Engine/StreamingLLM/model_draft.py:124)
 POOL_KERNEL = 5    # SnapKV avg-pool width (Engine/SnapKV/model.py:169)
-KV_DTYPES = {"bf16": torch.bfloat16, "fp8": ops.FP8_DTYPE}   # fp8 = OCP e4m3fn full-context cache
+# full-context caches: fp8 = OCP e4m3fn with static per-head scales; mxfp8, mxfp4 = 8- and 4-bit elements, a scale per 32 (ops.mx_kv_cache)
+KV_DTYPES = {"bf16": torch.bfloat16, "fp8": ops.FP8_DTYPE, "mxfp8": "mxfp8", "mxfp4": "mxfp4"}
+MX_SELECT_BYTES = 256 << 20      # of 16-bit keys and values that the SnapKV select of a block-scaled cache reads back at once
 FP8_MAX = 448.0
 FP8_MARGIN = 1.5
 
@@ -150,6 +152,11 @@ class RMSNorm(nn.Module):
         return ops.rmsnorm(x, self.weight, self.eps)
 
 
+def _is_mx(kvc, which):
+    """Is this the block-scaled one of a layer's caches?"""
+    return which == "kv_cache" and getattr(kvc, "mx", False)
+
+
 class KVCache(nn.Module):
     """Paged caches of one layer: `kv_cache` [pages, 2, 128, KH, D] and, for speculation, `draft_cache`."""
 
@@ -158,12 +165,18 @@ class KVCache(nn.Module):
         """kv_dtype=float8_e4m3fn stores `kv_cache` as OCP e4m3fn bytes with static per-kv-head scales
         (`k_scale`, `v_scale`, float32 [KH]; x ~ byte * scale); `draft_cache` is always bf16.
         kv_layout="HND" stores `kv_cache` as [pages, 2, KH, 128, D] (rows of a kv head contiguous: the streaming
-        reads of the verify step become 128-row runs); `draft_cache` is always NHD."""
+        reads of the verify step become 128-row runs); `draft_cache` is always NHD.
+        kv_dtype="mxfp8" / "mxfp4" stores it block-scaled, always HND."""
         super().__init__()
         if kv_layout not in ops.KV_LAYOUTS:
             raise ValueError(f"kv_layout must be one of {ops.KV_LAYOUTS}")
         self.layout = kv_layout
-        if max_num_pages > 0:
+        self.mx = kv_dtype in ("mxfp8", "mxfp4")
+        if self.mx and max_num_pages > 0:
+            if kv_layout != "HND":
+                raise ValueError(f"kv_dtype {kv_dtype} needs kv_layout HND, got {kv_layout}")
+            self.register_buffer("kv_cache", ops.mx_kv_cache(max_num_pages, n_heads, head_dim, kv_dtype, page_size, "cpu"), persistent=False)
+        elif max_num_pages > 0:
             shape = ((max_num_pages, 2, n_heads, page_size, head_dim) if kv_layout == "HND"
                      else (max_num_pages, 2, page_size, n_heads, head_dim))
             self.register_buffer("kv_cache", torch.zeros(shape, dtype=kv_dtype), persistent=False)
@@ -298,7 +311,7 @@ class Transformer(nn.Module):
             raise NotImplementedError("the gfx950 kernels are bf16")
         if kv_dtype not in KV_DTYPES:
             raise ValueError(f"kv_dtype must be one of {sorted(KV_DTYPES)}")
-        if (kv_dtype == "fp8" or kv_layout != "NHD") and streaming and not spec:
+        if (kv_dtype != "bf16" or kv_layout != "NHD") and streaming and not spec:
             raise NotImplementedError("the StreamingLLM ring cache is bf16 NHD only (in-place shift + re-rotation)")
         head_dim = c.dim // c.n_head
         self.page_size = page_size
@@ -825,6 +838,26 @@ class Transformer(nn.Module):
         dist.all_reduce(all_i, group=self.process_group)
         return ops.tp_argmax_merge(all_v, all_i)
 
+    def _select_mx(self, q_rot, cache, tab: PageTable, draft_cache, snap_tab: PageTable):
+        """The SnapKV select of a block-scaled cache: some requests' rows at a time read back (ops.read_kv) into 16-bit pages of their own."""
+        ctx, page, KH, D = self._snap_ctx_len, cache.shape[3], cache.shape[2], q_rot.shape[2]
+        B, each = tab.indptr.numel() - 1, -(-ctx // page)
+        most = max(1, min(B, MX_SELECT_BYTES // (each * page * KH * D * 4)))
+        dev = cache.device
+        k, v = (torch.empty((most * ctx, KH, D), dtype=torch.bfloat16, device=dev) for _ in (0, 1))
+        pages = torch.empty((most * each, 2, page, KH, D), dtype=torch.bfloat16, device=dev)
+        mine = torch.arange(most * each, dtype=torch.int32, device=dev)
+        for a in range(0, B, most):
+            n = min(most, B - a)
+            count = torch.arange(n + 1, dtype=torch.int32, device=dev)
+            rows, indptr, last = count * ctx, count * each, torch.full((n,), (ctx - 1) % page + 1, dtype=torch.int32, device=dev)
+            ops.read_kv(k[:n * ctx], v[:n * ctx], rows, cache, tab.indices, tab.indptr[a:a + n + 1], tab.last_page_len[a:a + n], n_max=ctx,
+                        kv_layout="HND")
+            ops.update_kv(k[:n * ctx], v[:n * ctx], rows, pages, mine, indptr, last, n_max=ctx)
+            ops.snapkv_select(q_rot[a * self.window_size:(a + n) * self.window_size], pages, mine, indptr, ctx, self.window_size,
+                              self.draft_budget, POOL_KERNEL, draft_cache, snap_tab.indices, snap_tab.indptr[a:a + n + 1],
+                              snap_tab.last_page_len[a:a + n], self.workspace)
+
     def _attend(self, q_rot, cache, qo_indptr, tab: PageTable, n, kv_scales=None, kv_layout="NHD"):
         return ops.paged_attention(q_rot, cache, qo_indptr, tab.indices, tab.indptr, tab.last_page_len, n,
                                    tab.max_pages, self.workspace, causal=True, kv_scales=kv_scales,
@@ -851,7 +884,7 @@ class Transformer(nn.Module):
             # consecutive rows (what every back-end passes: qo_indptr = arange * n); anything else takes rope_append, which
             # honours qo_indptr
             uniform_rows = idx.dim() == 2 and yin.shape[0] == (qo_indptr.numel() - 1) * n
-            if (not need_calib and uniform_rows and self._fused_here(yin, att.wqkv.weight, "qkv", pro is not None)
+            if (not need_calib and uniform_rows and not _is_mx(kvc, which) and self._fused_here(yin, att.wqkv.weight, "qkv", pro is not None)
                     and c.head_dim in (64, 128)):
                 # (deferred RMSNorm +) wqkv + bias + RoPE + paged append (both caches of a self-speculation verify):
                 # ONE launch
@@ -880,9 +913,12 @@ class Transformer(nn.Module):
             if snap_tab is not None:
                 if head_rows is not None:                 # the observation window is the prompt's last chunk
                     q_rot = q_rot.index_select(0, head_rows)
-                ops.snapkv_select(q_rot, cache, tab.indices, tab.indptr, self._snap_ctx_len, self.window_size,
-                                  self.draft_budget, POOL_KERNEL, kvc.draft_cache, snap_tab.indices, snap_tab.indptr,
-                                  snap_tab.last_page_len, self.workspace, kv_scales=scales, kv_layout=layout)
+                if _is_mx(kvc, which):
+                    self._select_mx(q_rot, cache, tab, kvc.draft_cache, snap_tab)
+                else:
+                    ops.snapkv_select(q_rot, cache, tab.indices, tab.indptr, self._snap_ctx_len, self.window_size,
+                                      self.draft_budget, POOL_KERNEL, kvc.draft_cache, snap_tab.indices, snap_tab.indptr,
+                                      snap_tab.last_page_len, self.workspace, kv_scales=scales, kv_layout=layout)
             return o
         return self._run(idx, fn, n_max, head_rows)
 

@@ -42,8 +42,9 @@ def _common(parser, script, kind=None):
     parser.add_argument('--seed', type=int, default=123, help='Random seed.')
     parser.add_argument('--printoutput', action='store_true', help='Whether to print the generated text.')
     parser.add_argument('--benchmark', action='store_true', help='Per-phase timing (adds synchronisations).')
-    parser.add_argument('--kv_dtype', type=str, default="bf16", choices=["bf16", "fp8"],
-                        help='Storage of the full-context KV cache (fp8 = OCP e4m3fn; not in the reference).')
+    parser.add_argument('--kv_dtype', type=str, default="bf16", choices=["bf16", "fp8", "mxfp8", "mxfp4"],
+                        help='Storage of the full-context KV cache (fp8 = OCP e4m3fn with static per-head scales; mxfp8, mxfp4 = 8- and 4-bit '
+                             'elements with a power-of-two scale for each 32; not in the reference).')
     parser.add_argument('--kv_layout', type=str, default=None, choices=["NHD", "HND"],
                         help='Page layout of the full-context KV cache.  Default: the Engine default '
                              '(backend_core.default_kv_layout(): HND -- the rows of one kv head contiguous inside a '
