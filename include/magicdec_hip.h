@@ -166,7 +166,7 @@ int md_paged_attn(const void* q, int64_t q_row_stride, const void* cache, void* 
 /* ------------------------------------------------------------------------
  * K13  block-scaled KV pages, rows read back, attention with a sliding window (no counterpart in the reference)
  * md_append_paged_kv and md_rope_append write block-scaled caches too (kv_dtype MD_KV_MXFP8 / MD_KV_MXFP4 | MD_KV_LAYOUT_HND; D 64 or 128,
- * page_size % 32 == 0).  Scales: per 32 elements of a row the smallest power of two at which no element is off by more than half a step of its
+ * page_size % 32 == 0, at most 65 536, as in the calls below).  Scales: per 32 elements of a row the smallest power of two at which no element is off by more than half a step of its
  * binade (elements round to nearest even, ties too), at least 2^-100; blocks with an infinity or a NaN read as NaN throughout.
  *
  * md_kv_row_bytes     bytes of one row of one kv head, scales included (0: no such cache)
@@ -175,7 +175,7 @@ int md_paged_attn(const void* q, int64_t q_row_stride, const void* cache, void* 
  *                     are left as they were.
  * md_window_attn      md_paged_attn (causal) of every kv_dtype, where a row at position t sees the positions s <= t with s > t - window or
  *                     s < sinks (window 0: all up to t).  A row that sees nothing is 0.  What is in a hidden place, infinities and NaN
- *                     included, has no effect on the rows that it is hidden from.  sm_scale > 0; page_size % 32 == 0; D 64 or 128.
+ *                     included, has no effect on the rows that it is hidden from.  sm_scale > 0; D 64 or 128.
  * workspace: md_window_attn_workspace_bytes(), 16-byte aligned, of this call alone until it has run.
  * ---------------------------------------------------------------------- */
 int md_kv_row_bytes(int kv_dtype, int D);

@@ -618,7 +618,7 @@ void launch_window_merge(const WinParams& p, int rows, hipStream_t st) {
 }
 
 bool window_shape_ok(int B, int n_max, int H, int KH, int max_pages, int page_size) {
-    return B > 0 && n_max > 0 && KH > 0 && H > 0 && H % KH == 0 && max_pages > 0 && page_size > 0 && page_size % 32 == 0 &&
+    return B > 0 && n_max > 0 && KH > 0 && H > 0 && H % KH == 0 && max_pages > 0 && page_size > 0 && page_size % 32 == 0 && page_size <= 65536 &&
            (int64_t)max_pages * page_size < (1 << 30) && (int64_t)n_max * (H / KH) < (1 << 30);
 }
 
@@ -636,7 +636,7 @@ extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* c
                               const float* k_scale, const float* v_scale, void* workspace, size_t workspace_bytes, md_stream_t stream) {
     MD_CHECK_ARG(q && cache && out && qo_indptr && page_indices && page_indptr && last_page_len, "md_window_attn: null pointer argument");
     MD_CHECK_ARG(window_shape_ok(B, n_max, H, KH, max_pages_per_req, page_size),
-                 "md_window_attn: bad shape B=%d n_max=%d H=%d KH=%d pages=%d page_size=%d (pages of multiples of 32 rows)", B, n_max, H, KH,
+                 "md_window_attn: bad shape B=%d n_max=%d H=%d KH=%d pages=%d page_size=%d (pages of multiples of 32 rows, to 65 536)", B, n_max, H, KH,
                  max_pages_per_req, page_size);
     if (D != 64 && D != 128) {
         md_set_error("md_window_attn: head_dim %d unsupported (64 or 128)", D);

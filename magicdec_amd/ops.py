@@ -119,6 +119,8 @@ def _kv_args(kv_cache, kv_scales, kv_layout="NHD", head_dim=None):
     if _is_mx(kv_cache):
         if kv_layout != "HND" or kv_scales is not None:
             raise ValueError("a block-scaled KV cache is HND and takes no kv_scales")
+        if head_dim is None:
+            raise ValueError("this operator takes no block-scaled KV cache (read_kv gives its rows)")
         kind = _MX_ROWS.get((head_dim, kv_cache.shape[4]))
         if kind is not None:
             return kind | flag, None, None
@@ -403,6 +405,8 @@ def _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_pa
         return out
     window, sinks = 0 if window is None else min(window, 1 << 30), min(sinks, 1 << 30)
     ws = workspace.get(_window_workspace(B, n_max, H, KH, D, max_pages_per_req, page_size, kind, window, sinks))
+    if ws.get_device() != cur:
+        raise ValueError(f"{what}: a workspace of {ws.device} while the current device is cuda:{cur}")
     check(_lib.load().md_window_attn(q.data_ptr(), q.stride(0), kv_cache.data_ptr(), out.data_ptr(), qo_indptr.data_ptr(),
                                      _pages(page_indices, page_indptr), page_indptr.data_ptr(), last_page_len.data_ptr(), B, n_max, H, KH, D,
                                      page_size, window, sinks, 1.0 / math.sqrt(D) if sm_scale is None else sm_scale, max_pages_per_req, kind, ks,

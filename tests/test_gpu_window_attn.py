@@ -41,9 +41,10 @@ def caches(kind, pages, KH, page, D, seed, ops, layout="HND", edit=None):
     return cache.to(DEV), scales, values
 
 
-def attend(ops, q, cache, rows, lens, page, tab, window, sinks, scales=None, layout="HND", ws=None, **more):
-    indices, indptr, last, _, most = tab
-    return ops.paged_attention(q.to(DEV), cache, mx.indptr_of(rows).to(DEV), indices.to(DEV), indptr.to(DEV), last.to(DEV), max(1, max(rows)), most,
+def attend(ops, q, cache, rows, lens, page, tab, window, sinks, scales=None, layout="HND", ws=None, n_max=None, most=None, **more):
+    indices, indptr, last = tab[:3]
+    return ops.paged_attention(q.to(DEV), cache, mx.indptr_of(rows).to(DEV), indices.to(DEV), indptr.to(DEV), last.to(DEV), n_max or max(1, max(rows)),
+                               most or tab[4],
                                ws or ops.AttnWorkspace(DEV), kv_scales=scales, kv_layout=layout, window=window or None, sinks=sinks, **more)
 
 
@@ -103,6 +104,91 @@ def test_against_64_bits(ops, kind, name, D, H, KH, page, lens, rows, window, si
     check(f"{kind}/{name}", out, want, size, mx.attention_bound(size, q, values))
 
 
+# Each way in which rows and keys are laid over workgroups: the bounds that a caller gives (rows and pages of a request, at most) choose it, whatever
+# lies in them.  (name, D, H, KH, page, tokens, new rows, window, sinks, n_max, pages)
+PLANS = [
+    ("row-groups-of-32", 64, 8, 4, 128, [60 + 5 * b for b in range(25)], [b % 21 for b in range(25)], 0, 0, 20, 1),
+    ("row-groups-of-32-d128", 128, 8, 4, 128, [60 + 5 * b for b in range(25)], [b % 21 for b in range(25)], 40, 3, 20, 2),
+    ("64-splits", 128, 8, 1, 128, [700], [2], 0, 0, 2, 700),
+    ("64-splits-tiles-of-64", 64, 8, 1, 128, [1500], [2], 0, 0, 2, 700),
+    ("64-splits-window", 64, 8, 1, 64, [1500, 3], [2, 1], 1000, 100, 2, 1400),
+    ("one-part-tiles-of-64", 64, 2, 2, 64, [800 + 3 * b for b in range(70)], [1] * 70, 0, 0, 1, 300),
+    ("4-waves-32-splits", 128, 4, 1, 128, [900], [30], 0, 0, 30, 300),
+    ("8-waves-32-splits", 128, 1, 1, 128, [700], [300], 0, 0, 300, 470),
+    ("8-waves-32-splits-d64", 64, 1, 1, 128, [700], [300], 100, 4, 300, 470),
+    ("8-waves-whole", 128, 2, 1, 128, [300, 150, 0, 260], [300, 131, 0, 257], 0, 0, 4000, 60),
+    ("8-waves-page-64", 128, 1, 1, 64, [700], [300], 0, 0, 300, 940),
+    ("8-waves-page-96", 128, 1, 1, 96, [700], [300], 130, 70, 300, 700),
+    ("8-waves-page-32-d64", 64, 1, 1, 32, [700], [300], 130, 7, 300, 1900),
+    ("4-waves-page-32", 128, 5, 1, 32, [300, 40], [13, 9], 0, 0, 13, 10),
+    ("4-waves-page-160", 128, 5, 1, 160, [400, 40], [13, 9], 50, 20, 13, 3),
+    ("4-waves-page-96-d64", 64, 5, 1, 96, [300, 40], [13, 9], 50, 20, 13, 4),
+    ("few-of-8-waves", 128, 4, 1, 128, [600, 200], [30, 32], 0, 0, 32, 5),
+    ("tokens-page-96", 128, 8, 2, 96, [300, 97, 5], [1, 2, 3], 0, 0, 3, 4),
+    ("far-more-rows-allowed", 64, 8, 2, 128, [300, 97, 5], [1, 2, 3], 0, 0, 2000, 4),
+]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("name,D,H,KH,page,lens,rows,window,sinks,n_max,most", PLANS, ids=[c[0] for c in PLANS])
+def test_every_layout_of_the_work(ops, kind, name, D, H, KH, page, lens, rows, window, sinks, n_max, most):
+    if kind in ("bf16", "fp8") and not window:
+        window = 1 << 20
+    tab = mx.table(lens, page, seed=len(name))
+    cache, scales, values = caches(kind, tab[3], KH, page, D, 5, ops)
+    # queries as a slice of a wider product's output
+    wide = (2 * torch.randn(sum(rows), H + 3, D, generator=torch.Generator().manual_seed(1))).to(BF)
+    q = wide[:, 1:H + 1]
+    want, size = mx.window_attention(q, values, lens, rows, tab[0], tab[1], window, sinks)
+    out = torch.full((sum(rows), H, D), 7.0, dtype=BF, device=DEV)
+    dq = wide.to(DEV)[:, 1:H + 1]
+    got = ops.paged_attention(dq, cache, mx.indptr_of(rows).to(DEV), *(t.to(DEV) for t in tab[:3]), n_max, most, ops.AttnWorkspace(DEV), out=out,
+                              kv_scales=scales, kv_layout="HND", window=window or None, sinks=sinks)
+    assert got.data_ptr() == out.data_ptr()
+    check(f"{kind}/{name}", got, want, size, mx.attention_bound(size, q, values))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("n", [1, 60])
+def test_rows_behind_the_last_request_stay(ops, kind, n):
+    """A batch padded behind its last request: those rows of the result are not written.  Requests that share pages read the same ones."""
+    D, H, KH, page = 64, 4, 2, 128
+    lens, rows = [300, 300], [n, n]
+    indices, indptr, last, pages, most = mx.table(lens, page)
+    indices[3:5] = indices[0:2]                                  # the second request's first pages are the first one's
+    cache, scales, values = caches(kind, pages, KH, page, D, 5, ops)
+    q = torch.randn(2 * n + 5, H, D, generator=torch.Generator().manual_seed(1)).to(BF)
+    out = torch.full((2 * n + 5, H, D), 7.0, dtype=BF, device=DEV)
+    ops.paged_attention(q.to(DEV), cache, mx.indptr_of(rows).to(DEV), indices.to(DEV), indptr.to(DEV), last.to(DEV), n, most, ops.AttnWorkspace(DEV),
+                        out=out, kv_layout="HND", window=290, sinks=2)
+    assert bool((out[2 * n:] == 7.0).all())
+    want, size = mx.window_attention(q[:2 * n], values, lens, rows, indices, indptr, 290, 2)
+    check(f"{kind}/shared pages", out[:2 * n], want, size, mx.attention_bound(size, q[:2 * n], values))
+
+
+def test_refusals_on_the_gpu(ops):
+    """What the wrapper refuses before a launch."""
+    D, H, KH, page = 128, 4, 2, 128
+    tab = mx.table([200], page)
+    cache, _, _ = caches("mxfp8", tab[3], KH, page, D, 5, ops)
+    q = torch.zeros(1, H, D, dtype=BF)
+    call = lambda q=q, cache=cache, tab=tab, **more: attend(ops, q, cache, [1], [200], page, tab, more.pop("window", 0), more.pop("sinks", 0), **more)  # noqa: E731
+    call()
+    for more in (dict(layout="NHD"), dict(causal=False), dict(sinks=-1), dict(window=-3), dict(scales=(q, q)), dict(q=torch.zeros(1, 3, D, dtype=BF)),
+                 dict(q=torch.zeros(1, H, 64, dtype=BF)), dict(q=torch.zeros(1, H, D)), dict(q=torch.zeros(1, H, 2 * D, dtype=BF, device=DEV)[..., ::2]),
+                 dict(out=torch.zeros(1, H, D, device=DEV)), dict(out=torch.zeros(2, H, D, dtype=BF, device=DEV))):
+        with pytest.raises(ValueError):
+            call(**more)
+    with pytest.raises(TypeError):
+        call(tab=(tab[0].long(), *tab[1:]))
+    with pytest.raises(ops.MagicDecHipError, match="sm_scale"):
+        call(sm_scale=-1.0)
+    for op in (lambda: ops.snapkv_select(q.to(DEV), cache, *(t.to(DEV) for t in tab[:2]), 200, 32, 64, 5, cache, *(t.to(DEV) for t in tab[:3]),
+                                         ops.AttnWorkspace(DEV), kv_layout="HND"),):
+        with pytest.raises(ValueError, match="block-scaled"):
+            op()
+
+
 def hidden_garbage(lens, rows, tab, page, window, sinks):
     """An edit of a cache that puts infinities, NaN and the largest numbers into every place that no row of the request sees."""
     indices, indptr = tab[0], tab[1]
@@ -143,11 +229,12 @@ def test_what_no_row_sees_has_no_effect(ops, kind, lens, rows, window, sinks, D)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "mxfp8", "mxfp4"])
-@pytest.mark.parametrize("n,D", [(4, 128), (40, 64), (130, 128), (300, 128)])
-def test_infinite_keys_and_values_reach_the_rows_that_see_them_alone(ops, kind, n, D):
+@pytest.mark.parametrize("n,D,window,most", [(4, 128, 150, None), (40, 64, 150, None), (130, 128, 150, None), (300, 128, 150, None),
+                                             (4, 64, 1 << 20, None), (300, 128, 1 << 20, 470), (300, 64, 1 << 20, 470)])
+def test_infinite_keys_and_values_reach_the_rows_that_see_them_alone(ops, kind, n, D, window, most):
     """The token at position p of a chunk has a NaN in its key, another an infinity in its value: rows before them are as without, rows behind
     the key's are NaN, rows that see the value are not finite in its place (block-scaled: its block)."""
-    H, KH, page, past, window, sinks = 4, 1, 128, 200, 150, 2
+    H, KH, page, past, sinks = 4, 1, 128, 200, 2
     lens, rows = [past + n], [n]
     tab = mx.table(lens, page)
     nan_at, inf_at = past + n - 1, past + n // 2
@@ -160,8 +247,8 @@ def test_infinite_keys_and_values_reach_the_rows_that_see_them_alone(ops, kind, 
     q = torch.randn(n, H, D, generator=torch.Generator().manual_seed(1)).to(BF)
     cache, _, _ = caches(kind, tab[3], KH, page, D, 5, ops, edit=edit)
     clean, _, _ = caches(kind, tab[3], KH, page, D, 5, ops)
-    a = attend(ops, q, cache, rows, lens, page, tab, window, sinks).cpu()
-    c = attend(ops, q, clean, rows, lens, page, tab, window, sinks).cpu()
+    a = attend(ops, q, cache, rows, lens, page, tab, window, sinks, most=most).cpu()
+    c = attend(ops, q, clean, rows, lens, page, tab, window, sinks, most=most).cpu()
     first = n // 2                                              # rows from here on see the value
     assert torch.equal(a[:first], c[:first])
     assert bool(a[n - 1].isnan().all())

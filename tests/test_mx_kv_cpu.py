@@ -49,6 +49,7 @@ def attend(kind=MX8 | HND, D=128, page=128, q=P, B=2, n=4, H=8, KH=2, stride=102
     (attend, dict(scale=0.0), INVALID, "sm_scale"), (attend, dict(scale=float("nan")), INVALID, "sm_scale"), (attend, dict(kind=FP8), INVALID, "scales"),
     (attend, dict(kind=0x400), INVALID, "flags"), (attend, dict(stride=1025), INVALID, "aligned"), (attend, dict(q=None), INVALID, "null"),
     (attend, dict(n=0), INVALID, "n_max=0"), (attend, dict(pages=0), INVALID, "pages=0"),
+    (append, dict(page=131072), INVALID, "65 536"), (read, dict(page=131072), INVALID, "65 536"), (attend, dict(page=131072), INVALID, "65 536"),
     (attend, dict(B=1, KH=1, pages=200, ws=None), WORKSPACE, "workspace"), (attend, dict(B=1, KH=1, pages=200, ws_bytes=100), WORKSPACE, "workspace"),
 ])
 def test_the_library_refuses(call, args, code, words):
@@ -86,6 +87,8 @@ def test_python_refuses_on_the_cpu():
         ops._kv_args(cache, None, "NHD", 64)
     with pytest.raises(ValueError, match="kv_scales"):
         ops._kv_args(cache, (i, i), "HND", 64)
+    with pytest.raises(ValueError, match="no block-scaled"):
+        ops._kv_args(cache, None, "HND")
     with pytest.raises(ValueError, match="66 bytes"):
         ops._kv_args(cache, None, "HND", 128)
     assert ops._kv_args(cache, None, "HND", 64) == (MX8 | HND, None, None)
