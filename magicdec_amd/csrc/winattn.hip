@@ -24,7 +24,7 @@ namespace {
 
 template <int D, int QT, int KG>
 __host__ __device__ constexpr int win_wave_lds() {
-    const int image = KG * (D / 16) * kVSub, merge = QT * D * 64 + QT * 128;
+    const int image = KG * (D / 16) * kVSub, merge = QT * 16 * (D + 4) * 4 + QT * 128;
     return ((image > merge ? image : merge) + 255) / 256 * 256;
 }
 
@@ -66,25 +66,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     const int kv_len = min(kv_len_of(p.indptr, p.last, b, p.page_size, &pg0, &room), room);
     const int nrows = n_b * g;
 
-    // a lane's query rows see up to lim, and of those up to low only the first tokens
+    // a lane's query rows see up to lim, and of those up to low only the first tokens; lo, hi: the first and the last row's lim
     int lim[QT], low[QT];
-    int hi = -1, lo = 0x7fffffff;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         const int R = (qg * QT + qt) * 16 + lq;
-        const bool valid = R < nrows;
-        lim[qt] = valid ? kv_len - n_b + R / g : -1;
+        lim[qt] = R < nrows ? kv_len - n_b + R / g : -1;
         low[qt] = p.window > 0 ? lim[qt] - p.window : -1;
-        hi = max(hi, lim[qt]);
-        if (valid) lo = min(lo, lim[qt]);
     }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) {
-        hi = max(hi, __shfl_xor(hi, o));
-        lo = min(lo, __shfl_xor(lo, o));
-    }
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int first = qg * QT * 16, last = min(first + QT * 16, nrows) - 1;
+    if (last < first) return;
+    const int lo = kv_len - n_b + first / g, hi = kv_len - n_b + last / g;
     const int hi_low = p.window > 0 ? hi - p.window : -1;
     const Tiles tiles(lo, min(hi + 1, kv_len), p.window, p.sinks, KT);
     const int per = (tiles.count + p.nsplit - 1) / p.nsplit;
@@ -387,42 +379,44 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
         l[qt] += __shfl_xor(l[qt], 32);
     }
     __syncthreads();
+    // rows of sums, 4 numbers apart from whole banks: 16 lanes write and read different ones
+    constexpr int ROWS = QT * 16, PITCH = D + 4;
     float* mo = reinterpret_cast<float*>(smem + wave * WAVE_LDS);
-    float* mst = mo + QT * D * 16;
+    float* mst = mo + ROWS * PITCH;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) mo[(qt * D + nb * 16 + ((SWAP && nb >= 4) ? (lc ^ 2) : lc) * 4 + r) * 16 + lq] = o[qt][nb][r];
+            *reinterpret_cast<f32x4*>(mo + (qt * 16 + lq) * PITCH + nb * 16 + ((SWAP && nb >= 4) ? (lc ^ 2) : lc) * 4) = o[qt][nb];
         if (lc == 0) {
             mst[(qt * 16 + lq) * 2] = m[qt];
             mst[(qt * 16 + lq) * 2 + 1] = l[qt];
         }
     }
     __syncthreads();
-    constexpr int ROWS = QT * 16;
-    for (int e = tid; e < ROWS * D; e += 64 * kWaves) {
-        const int Rl = e / D, d = e - Rl * D, R = qg * ROWS + Rl;
-        if (R >= nrows) continue;
-        const int qt = Rl >> 4, qq = Rl & 15;
-        float M = kLowest, L = 0.f, acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const float*>(smem + w * WAVE_LDS)[QT * D * 16 + (qt * 16 + qq) * 2]);
+    for (int e = tid; e < ROWS * (D / 4); e += 64 * kWaves) {
+        const int Rl = e / (D / 4), d = e % (D / 4) * 4, R = first + Rl;
+        if (R > last) break;                                     // (rows ascend with e)
+        float M = kLowest, L = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) M = fmaxf(M, reinterpret_cast<const float*>(smem + w * WAVE_LDS)[ROWS * PITCH + Rl * 2]);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
             const float* ow = reinterpret_cast<const float*>(smem + w * WAVE_LDS);
-            const float* sw = ow + QT * D * 16 + (qt * 16 + qq) * 2;
-            const float a = __builtin_amdgcn_exp2f(sw[0] - M);
-            L += sw[1] * a;
-            acc += ow[(qt * D + d) * 16 + qq] * a;
+            const float a = __builtin_amdgcn_exp2f(ow[ROWS * PITCH + Rl * 2] - M);
+            L += ow[ROWS * PITCH + Rl * 2 + 1] * a;
+            acc += *reinterpret_cast<const f32x4*>(ow + Rl * PITCH + d) * a;
         }
         if (p.nsplit == 1) {
             const int qi = R / g;
-            p.out[((int64_t)(q0 + qi) * p.H + kvh * g + R - qi * g) * D + d] = f32_to_bf16(L == 0.f ? 0.f : acc * (vsc / L));
+            const float inv = L == 0.f ? 0.f : vsc / L;
+            if (L == 0.f) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+            *reinterpret_cast<bf16x4*>(p.out + ((int64_t)(q0 + qi) * p.H + kvh * g + R - qi * g) * D + d) = __builtin_convertvector(acc * inv, bf16x4);
         } else {
             const int64_t slot = (((int64_t)pair * p.n_qgroups + qg) * p.nsplit + split) * ROWS + Rl;
-            p.ws_o[slot * D + d] = acc;
+            *reinterpret_cast<f32x4*>(p.ws_o + slot * D + d) = acc;
             if (d == 0) {
                 p.ws_ml[slot * 2] = M;
                 p.ws_ml[slot * 2 + 1] = L;

@@ -34,10 +34,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     constexpr int PIECE = KIND == MD_KV_BF16 ? 8 : KIND == MD_KV_MXFP4 ? 32 : 16;      // elements of a piece
     constexpr int KROW = D * 2 + 16, K_BYTES = KT * KROW, VG = NB * kVSub, IMAGE = prompt_image_bytes<D, KT>();
 
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // 2 images; lowest, highest position of a wavefront; infinite values
-    int* s_lo = reinterpret_cast<int*>(smem + 2 * IMAGE);
-    int* s_hi = s_lo + NW;
-    int* s_infinite = s_hi + NW;                                             // [2][NW]
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];      // 2 images; [2][NW]: does an image have infinite values
+    int* s_infinite = reinterpret_cast<int*>(smem + 2 * IMAGE);
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63;
@@ -56,27 +54,10 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     const bool valid = R < nrows;
     const int qi = R / g, qr = R - qi * g;
     const int lim = valid ? kv_len - n_b + qi : -1, low = p.window > 0 ? lim - p.window : -1;
-    int hi = lim, lo = valid ? lim : 0x7fffffff;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        hi = max(hi, __shfl_xor(hi, o));
-        lo = min(lo, __shfl_xor(lo, o));
-    }
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    if (lane == 0) {
-        s_lo[wave] = lo;
-        s_hi[wave] = hi;
-    }
-    __syncthreads();
-    int lo_all = 0x7fffffff, hi_all = -1;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        lo_all = min(lo_all, s_lo[w]);
-        hi_all = max(hi_all, s_hi[w]);
-    }
-    lo_all = __builtin_amdgcn_readfirstlane(lo_all);
-    hi_all = __builtin_amdgcn_readfirstlane(hi_all);
+    // lo, hi: of the wavefront's first and last row; of the workgroup's
+    const int first = qg * NW * 32, last = min(first + NW * 32, nrows) - 1, first_w = first + wave * 32, last_w = min(first_w + 32, nrows) - 1;
+    const int lo_all = kv_len - n_b + first / g, hi_all = kv_len - n_b + last / g;
+    const int lo = first_w <= last_w ? kv_len - n_b + first_w / g : 0x7fffffff, hi = first_w <= last_w ? kv_len - n_b + last_w / g : -1;
     const Tiles tiles(lo_all, min(hi_all + 1, kv_len), p.window, p.sinks, KT);
     const int per = (tiles.count + p.nsplit - 1) / p.nsplit, t_begin = split * per, t_end = min(tiles.count, t_begin + per);
     // does a tile that begins at `pos` hide a key from a row between two positions; does any of them see one
@@ -375,7 +356,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
 
 template <int D, int NW, int KT>
 int launch_prompt(const WinParams& p, int grid, hipStream_t st) {
-    constexpr int lds = std::max(2 * prompt_image_bytes<D, KT>() + 4 * NW * 4, NW * 32 * D * 2);
+    constexpr int lds = std::max(2 * prompt_image_bytes<D, KT>() + 2 * NW * 4, NW * 32 * D * 2);
     auto k = window_prompt_kernel<D, NW, KT, MD_WIN_KIND>;
     if constexpr (lds > 64 * 1024) {
         static MdPerDeviceOnce once;
