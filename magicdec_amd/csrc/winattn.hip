@@ -505,48 +505,67 @@ struct WinPlan {
     size_t slots;
 };
 
+// What a way of laying out more than 32 rows a kv head is expected to take, in us: workgroups of `rows` rows walk their keys in steps of `unit`, in `parts`
+// of them.  A step takes `tau` while a CU has one workgroup, and `full` for each of the most that one has; a second launch joins parts, whose sums are
+// written and read back.  The numbers are fitted to 192 shapes, one request to 64 of 40 to 4 096 rows over 500 to 16 000 keys, in every way and number of
+// parts: what this picks takes 2 % more than the best of them on average.
+struct WinWay {
+    int nw, rows, unit;
+    double fixed, tau, full;
+    double us(int64_t workgroups, int64_t keys, int64_t parts, double sums) const {
+        const double steps = (double)((keys + unit * parts - 1) / (unit * parts)), most = (double)((workgroups + 255) / 256);
+        return fixed + steps * std::max(tau, full * most) + (parts > 1 ? 2.6 + sums * parts / 5e6 : 0.);
+    }
+};
+
 // All in us, 8 kv heads unless said.
 WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int page_size, int kind, int window, int sinks) {
     WinPlan pl;
     const int64_t rows = (int64_t)n_max * (H / KH), pairs = (int64_t)B * KH;
-    // keys that one row looks at, and those that neighbouring ones do besides, at most
+    // keys that a group of rows looks at, at most
     const int64_t all = (int64_t)max_pages * page_size;
-    const auto seen = [&](int64_t n) { return window > 0 ? std::min<int64_t>(all, (int64_t)window + n + std::min<int64_t>(sinks, all)) : all; };
-    const auto groups = [&](int64_t n) { return pairs * ((rows + n - 1) / n); };
-    // More than 32 rows: in workgroups of 8 wavefronts where those are many or walk far (512 x 4 heads over 4 000 keys of 128 in bf16: 60 in
-    // workgroups of 4, 54 of 8; over 700 keys 27 and 31), or where one of them, of larger tiles, does what one of 4 did (16 x 32 x 4 over 600 22,
-    // 28 of 4).  In groups of 32 on the kernel above, which shares a group's keys over its wavefronts, where these fill the chip by themselves and
-    // walk a short way: 16 requests x 10 x 4 heads over 600 keys 20, 24 in workgroups of 4; 512 x 4 of 64 over 700 17, 21; but 4 x 128 x 4 of 128
-    // over 600 in bf16 30, 26
-    const int64_t of32 = groups(32), walk = groups(256) * seen(n_max);
-    const bool short_way = seen(rows) <= 768 && of32 >= 200 && of32 <= 512 && (D == 64 || rows <= 64);
-    pl.nw = rows <= 32 || short_way ? 0 : rows >= 256 ? (walk >= 100000 ? 8 : 4) : rows > 96 && rows <= 128 && D == 128 && walk < 100000 ? 8 : 4;
-    pl.rows = pl.nw ? pl.nw * 32 : rows <= 16 ? 16 : 32;
+    const auto seen = [&](int64_t of) {
+        const int64_t n = std::min<int64_t>(n_max, (of + H / KH - 1) / (H / KH) + 1);
+        return window > 0 ? std::min<int64_t>(all, (int64_t)window + n + std::min<int64_t>(sinks, all)) : all;
+    };
+    pl.nw = 0;
+    pl.rows = rows <= 16 ? 16 : 32;
+    if (rows > 32) {
+        // the kernel above, whose wavefronts share a group's keys, so that keys are read and unpacked for every 32 rows; 4 and 8 wavefronts of winprompt.hip,
+        // which share them all
+        const int bits = kind == MD_KV_BF16 ? 16 : kind == MD_KV_MXFP4 ? 4 : 8;
+        const WinWay wide[3] = {{0, 32, 128, bits == 16 ? 6.7 : 8.2, bits == 4 ? 1.16 : 1.36, bits == 16 ? 2.2 : bits == 8 ? 1.37 : 1.06},
+                                {4, 128, 64, 7.7, 1.78, 1.27}, {8, 256, 128, 10.8, 3.2, 3.2}};
+        const WinWay narrow[3] = {{0, 32, 128, 6.4, 0.9, bits == 16 ? 1.03 : bits == 8 ? 0.83 : 0.66}, {4, 128, 64, 6.8, 1.18, 0.77}, {8, 256, 64, 8.1, 1.35, 1.05}};
+        const double sums = (double)(pairs * rows) * (D * 8 + 16);
+        double least = 1e300;
+        for (const WinWay& w : D == 64 ? narrow : wide) {
+            const int64_t groups = pairs * ((rows + w.rows - 1) / w.rows), keys = seen(w.rows);
+            for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+                if (parts > 1 && (keys < 128 * parts || groups * parts > 1024)) break;
+                const double us = w.us(groups * parts, keys, parts, sums);
+                if (us < least) least = us, pl.nw = w.nw, pl.rows = w.rows, pl.nsplit = parts;
+            }
+        }
+    }
     pl.n_qgroups = (int)((rows + pl.rows - 1) / pl.rows);
-    const int64_t keys = seen(std::min<int64_t>(n_max, (pl.rows + H / KH - 1) / (H / KH) + 1)), have = pairs * pl.n_qgroups;
-    // Keys over several workgroups, of enough keys each to pay for the launch that joins them (3.5).
-    int64_t want, most;
-    if (pl.nw) {
-        // one a CU, or what it holds of them where there are many: 4 x 10 x 4 rows over 4 000 keys 27 in 256, 29 in 512; 16 x 10 x 4 78 in 256, 57 in 512
-        const bool many = have >= 96;
-        want = (!many || pl.nw == 8 ? 256 : D == 64 ? 1024 : 512) / have, most = many ? keys / 1024 + 1 : pl.nw == 8 ? (keys + 255) / 256 : (keys + 159) / 160;
-    } else if (rows > 32) {
-        want = most = 1;
-    } else {
-        // One a CU up to half as many (4 x 4 rows over 5 000 keys in bf16: 70 whole, 22 in 256, 25 in 512), two where 8- or 4-bit streams stay long
-        // (8 x 4 over 8 000 37 and 34); beyond that three where streams are long (32 x 4 over 9 000 120 whole, 110), and so where the last
-        // workgroups would leave CUs behind (40 x 4 over 9 000 in bf16 311 whole, 242 in three; 48 x 4 337 and 289 in two)
+    const int64_t keys = seen(pl.rows), have = pairs * pl.n_qgroups;
+    if (rows <= 32) {
+        // Keys over several workgroups, of enough keys each to pay for the launch that joins them (3.5).  One a CU up to half as many (4 x 4 rows over 5 000
+        // keys in bf16: 70 whole, 22 in 256, 25 in 512), two where 8- or 4-bit streams stay long (8 x 4 over 8 000 37 and 34); beyond that
+        // three where streams are long (32 x 4 over 9 000 120 whole, 110), and so where the last workgroups would leave CUs behind (40 x 4 over
+        // 9 000 in bf16 311 whole, 242 in three; 48 x 4 337 and 289 in two)
         const int64_t stream = keys * 2 * kv_row_bytes(kind, D);
         const bool long_way = stream >= 700000, left = have * 100 < (have + 511) / 512 * 512 * 85;
+        int64_t want;
         if (have <= 128)
             want = (kind != MD_KV_BF16 && keys * have >= 512000 ? 512 : 256) / have;
         else if (have <= 256)
             want = kind != MD_KV_BF16 && long_way ? 768 / have : 1;
         else
             want = !long_way || !left ? 1 : have <= 352 ? 3 : 2;
-        most = keys <= 512 ? 1 : keys / 128;
+        pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, keys <= 512 ? 1 : keys / 128, 64}));
     }
-    pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, most, pl.nw ? 32 : 64}));
     // 64 keys at a time where that spills nothing and the stream is long: 4-bit heads of 64, 64 requests of 16 036 keys x 16 rows 133 -> 114, of 1 000 12.9
     // -> 12.2; one request of 1 500 in eight parts 8.5 -> 9.9
     pl.kg = kind == MD_KV_MXFP4 && D == 64 && pl.rows == 16 && page_size % 64 == 0 && keys / pl.nsplit >= 1024 ? 2 : 1;
