@@ -54,10 +54,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     const int lane = tid & 63;
     const int lq = lane & 15, lc = lane >> 4;
 
-    // workgroups of one (request, kv head) differ by multiples of 8: they share an XCD's L2
-    const int nsub = p.n_qgroups * p.nsplit;
-    const int sub = (blockIdx.x >> 3) % nsub, pair = ((blockIdx.x >> 3) / nsub) * 8 + (blockIdx.x & 7);
-    if (pair >= p.B * p.KH) return;
+    int sub;
+    const int pair = win_pair(p, p.n_qgroups * p.nsplit, sub);
     const int qg = sub / p.nsplit, split = sub % p.nsplit;
     const int b = pair / p.KH, kvh = pair % p.KH;
     const int g = p.group;
@@ -672,7 +670,7 @@ extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* c
         md_set_error("md_window_attn: workspace too small or misaligned (%zu < %zu)", workspace_bytes, need);
         return MD_ERR_WORKSPACE;
     }
-    const int64_t grid = (int64_t)(B * (int64_t)KH + 7) / 8 * 8 * pl.n_qgroups * pl.nsplit;
+    const int64_t grid = (int64_t)B * KH * pl.n_qgroups * pl.nsplit;
     MD_CHECK_ARG(grid <= 0x7fffffff, "md_window_attn: too many rows for a grid");
     WinParams p = {};
     p.q = (const bf16_t*)q;

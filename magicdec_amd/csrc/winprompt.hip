@@ -41,10 +41,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     const int lane = tid & 63;
     const int j = lane & 31, kh = lane >> 5;
 
-    const int sub = (blockIdx.x >> 3) % (p.n_qgroups * p.nsplit), split = sub % p.nsplit;
-    const int pair = ((blockIdx.x >> 3) / (p.n_qgroups * p.nsplit)) * 8 + (blockIdx.x & 7);
+    int sub;
+    const int pair = win_pair(p, p.n_qgroups * p.nsplit, sub), split = sub % p.nsplit;
     const int qg = p.n_qgroups - 1 - sub / p.nsplit;             // the last rows, with the most keys, first
-    if (pair >= p.B * p.KH) return;
     const int b = pair / p.KH, kvh = pair % p.KH, g = p.group;
     const int q0 = p.qo_indptr[b], n_b = p.qo_indptr[b + 1] - q0, nrows = n_b * g;
     if (qg * NW * 32 >= nrows) return;
