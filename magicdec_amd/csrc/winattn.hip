@@ -504,15 +504,16 @@ struct WinPlan {
 };
 
 // What a way of laying out more than 32 rows a kv head is expected to take, in us: workgroups of `rows` rows walk their keys in steps of `unit`, in `parts`
-// of them.  A step takes `tau` while a CU has one workgroup, and `full` for each of the most that one has; a second launch joins parts, whose sums are
-// written and read back.  The numbers are fitted to 192 shapes, one request to 64 of 40 to 4 096 rows over 500 to 16 000 keys, in every way and number of
-// parts: what this picks takes 2 % more than the best of them on average.
+// of them.  A step takes `tau` while a CU has one workgroup, and `full` for each of the most that one has; where it holds one at a time, each after the
+// first begins with `next`.  A window's ends and its first tokens are steps of their own.  A second launch joins parts, whose sums are written and read
+// back.  The numbers are fitted to 237 shapes, one request to 64 of 40 to 32 000 rows over 10 to 16 000 keys, in every way and number of parts: what this
+// picks takes 2 to 3 % more than the best of them on average.
 struct WinWay {
     int nw, rows, unit;
-    double fixed, tau, full;
-    double us(int64_t workgroups, int64_t keys, int64_t parts, double sums) const {
-        const double steps = (double)((keys + unit * parts - 1) / (unit * parts)), most = (double)((workgroups + 255) / 256);
-        return fixed + steps * std::max(tau, full * most) + (parts > 1 ? 2.6 + sums * parts / 5e6 : 0.);
+    double fixed, tau, full, next;
+    double us(int64_t workgroups, int64_t keys, int edges, int64_t parts, double sums) const {
+        const double steps = (double)(((keys + unit - 1) / unit + edges + parts - 1) / parts), most = (double)((workgroups + 255) / 256);
+        return fixed + (most - 1) * next + steps * std::max(tau, full * most) + (parts > 1 ? 2.6 + sums * parts / 5e6 : 0.);
     }
 };
 
@@ -532,16 +533,18 @@ WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int p
         // the kernel above, whose wavefronts share a group's keys, so that keys are read and unpacked for every 32 rows; 4 and 8 wavefronts of winprompt.hip,
         // which share them all
         const int bits = kind == MD_KV_BF16 ? 16 : kind == MD_KV_MXFP4 ? 4 : 8;
-        const WinWay wide[3] = {{0, 32, 128, bits == 16 ? 6.7 : 8.2, bits == 4 ? 1.16 : 1.36, bits == 16 ? 2.2 : bits == 8 ? 1.37 : 1.06},
-                                {4, 128, 64, 7.7, 1.78, 1.27}, {8, 256, 128, 10.8, 3.2, 3.2}};
-        const WinWay narrow[3] = {{0, 32, 128, 6.4, 0.9, bits == 16 ? 1.03 : bits == 8 ? 0.83 : 0.66}, {4, 128, 64, 6.8, 1.18, 0.77}, {8, 256, 64, 8.1, 1.35, 1.05}};
+        const WinWay wide[3] = {{0, 32, 128, bits == 16 ? 6.7 : 8.2, bits == 4 ? 1.16 : 1.36, bits == 16 ? 2.2 : bits == 8 ? 1.37 : 1.06, 0},
+                                {4, 128, 64, 7.7, 1.78, 1.27, 0}, {8, 256, 128, 10.8, 3.2, 3.2, 8}};
+        const WinWay narrow[3] = {{0, 32, 128, 6.4, 0.9, bits == 16 ? 1.03 : bits == 8 ? 0.83 : 0.66, 0},
+                                  {4, 128, 64, 6.8, 1.18, 0.77, 0}, {8, 256, 64, 8.1, 1.35, 1.05, 3}};
         const double sums = (double)(pairs * rows) * (D * 8 + 16);
         double least = 1e300;
         for (const WinWay& w : D == 64 ? narrow : wide) {
             const int64_t groups = pairs * ((rows + w.rows - 1) / w.rows), keys = seen(w.rows);
+            const int edges = keys == all ? 0 : 1 + (sinks > 0);
             for (int parts : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
                 if (parts > 1 && (keys < 128 * parts || groups * parts > 1024)) break;
-                const double us = w.us(groups * parts, keys, parts, sums);
+                const double us = w.us(groups * parts, keys, edges, parts, sums);
                 if (us < least) least = us, pl.nw = w.nw, pl.rows = w.rows, pl.nsplit = parts;
             }
         }
