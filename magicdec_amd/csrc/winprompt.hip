@@ -66,14 +66,6 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     auto sees = [&](int pos) { return pos <= hi && (p.window <= 0 || pos + KT - 1 > lo - p.window || pos < p.sinks); };
 
     bf16x8 qf[KS];
-    {
-        const bf16_t* qp = p.q + (int64_t)(q0 + qi) * p.q_row_stride + (kvh * g + qr) * D;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-            qf[ks] = valid ? *reinterpret_cast<const bf16x8*>(qp + ks * 16 + kh * 8) : z;
-        }
-    }
     const float sl2 = KIND == MD_KV_FP8_E4M3 ? p.scale_log2 * p.k_scale[kvh] : p.scale_log2;
     f32x16 o[DB];
 #pragma unroll
@@ -294,6 +286,15 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     };
 
     if (t_begin < t_end) issue(t_begin);
+    // behind the first tile's loads, which wait for the numbers of their pages
+    {
+        const bf16_t* qp = p.q + (int64_t)(q0 + qi) * p.q_row_stride + (kvh * g + qr) * D;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            qf[ks] = valid ? *reinterpret_cast<const bf16x8*>(qp + ks * 16 + kh * 8) : z;
+        }
+    }
     for (int i = t_begin; i < t_end; ++i) {
         unsigned char* img = smem + (i & 1) * IMAGE;
         const int pos0 = tiles.at(i) * KT;
