@@ -245,7 +245,8 @@ int md_mx_append(const void* q, const void* k, const void* v, int64_t qs, int64_
                  const int32_t* page_indptr2, const int32_t* last2, int page_size, int kv_dtype, hipStream_t stream, const char* what) {
     const int kind = kv_dtype & MD_KV_DTYPE_MASK;
     MD_CHECK_ARG(kv_dtype & MD_KV_LAYOUT_HND, "%s: block-scaled pages are HND", what);
-    MD_CHECK_ARG(B <= 65535 && H >= 0 && page_size % 32 == 0 && page_size <= 65536, "%s: bad shape B=%d H=%d page_size=%d (pages of multiples of 32 rows, to 65 536)", what, B, H, page_size);
+    MD_CHECK_ARG(B <= 65535 && n_max <= 1 << 30 && H >= 0 && page_size % 32 == 0 && page_size <= 65536,
+                 "%s: bad shape B=%d n_max=%d H=%d page_size=%d (pages of multiples of 32 rows, to 65 536)", what, B, n_max, H, page_size);
     if (D != 64 && D != 128) {
         md_set_error("%s: head_dim %d of a block-scaled cache unsupported (64 or 128)", what, D);
         return MD_ERR_UNSUPPORTED;
@@ -301,7 +302,7 @@ extern "C" int md_read_paged_kv(void* k_out, void* v_out, int64_t k_row_stride, 
                                 const int32_t* page_indices, const int32_t* page_indptr, const int32_t* last_page_len, int B, int n_max, int KH,
                                 int D, int page_size, int kv_dtype, const float* k_scale, const float* v_scale, md_stream_t stream) {
     MD_CHECK_ARG(k_out && v_out && indptr && cache && page_indices && page_indptr && last_page_len, "md_read_paged_kv: null pointer argument");
-    MD_CHECK_ARG(B > 0 && B <= 65535 && n_max > 0 && KH > 0 && page_size > 0 && page_size % 32 == 0 && page_size <= 65536,
+    MD_CHECK_ARG(B > 0 && B <= 65535 && n_max > 0 && n_max <= 1 << 30 && KH > 0 && page_size > 0 && page_size % 32 == 0 && page_size <= 65536,
                  "md_read_paged_kv: bad shape B=%d n_max=%d KH=%d page_size=%d (pages of multiples of 32 rows, to 65 536)", B, n_max, KH, page_size);
     if (D != 64 && D != 128) {
         md_set_error("md_read_paged_kv: head_dim %d unsupported (64 or 128)", D);

@@ -50,6 +50,7 @@ def attend(kind=MX8 | HND, D=128, page=128, q=P, B=2, n=4, H=8, KH=2, stride=102
     (attend, dict(kind=0x400), INVALID, "flags"), (attend, dict(stride=1025), INVALID, "aligned"), (attend, dict(q=None), INVALID, "null"),
     (attend, dict(n=0), INVALID, "n_max=0"), (attend, dict(pages=0), INVALID, "pages=0"),
     (append, dict(page=131072), INVALID, "65 536"), (read, dict(page=131072), INVALID, "65 536"), (attend, dict(page=131072), INVALID, "65 536"),
+    (append, dict(n=2147483647), INVALID, "n_max=2147483647"), (read, dict(n=2147483647), INVALID, "n_max=2147483647"),
     (attend, dict(B=1, KH=1, pages=200, ws=None), WORKSPACE, "workspace"), (attend, dict(B=1, KH=1, pages=200, ws_bytes=100), WORKSPACE, "workspace"),
 ])
 def test_the_library_refuses(call, args, code, words):
