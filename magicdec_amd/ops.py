@@ -217,6 +217,8 @@ def read_kv(k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_las
         raise ValueError(f"{what}: {rows} rows of k and {v.shape[0]} of v")
     if width != D and not _is_mx(kv_cache):
         raise ValueError(f"{what}: rows of {D} elements of a cache of {width}")
+    if rows > 1 and min(k.stride(0), v.stride(0)) < KH * D:
+        raise ValueError(f"{what}: k and v are written: rows that share memory")
     if B >= 1 and rows:
         check(_lib.load().md_read_paged_kv(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), indptr.data_ptr(), kv_cache.data_ptr(),
                                            _pages(kv_page_indices, kv_page_indptr), kv_page_indptr.data_ptr(), kv_page_lastlen.data_ptr(), B,

@@ -195,3 +195,19 @@ def test_pages_behind_four_gib(ops):
     a = ops.paged_attention(q, cache, qo, ix, pi, la, 4, 3, ws, kv_layout="HND")
     c = ops.paged_attention(q, small, qo, low, pi, la, 4, 3, ws, kv_layout="HND")
     assert torch.equal(a, c)
+
+
+def test_read_kv_refuses_rows_that_share_memory(ops):
+    """An expanded row can be appended many times, but not be written as many."""
+    D, KH, page = 64, 2, 128
+    cache = ops.mx_kv_cache(1, KH, D, "mxfp8")
+    table = [torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 3], [0], [0, 1], [3])]
+    one = torch.randn(1, KH, D, generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    many, out = one.expand(3, KH, D), torch.zeros(3, KH, D, dtype=BF, device=DEV)
+    ops.update_kv(many, many, table[0], cache, *table[1:], kv_layout="HND")
+    for k, v in ((many, out), (out, many)):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.read_kv(k, v, table[0], cache, *table[1:], kv_layout="HND")
+    k, v = ops.read_kv(out, torch.zeros_like(out), table[0], cache, *table[1:], kv_layout="HND")
+    assert torch.equal(k[0], k[2]) and torch.equal(v, k)
+    assert bool(((k[0] - one[0]).abs() <= one.abs().amax() / 16).all())
