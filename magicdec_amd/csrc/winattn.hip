@@ -694,8 +694,8 @@ extern "C" int md_window_attn(const void* q, int64_t q_row_stride, const void* c
     p.page_size = page_size;
     p.nsplit = pl.nsplit;
     p.n_qgroups = pl.n_qgroups;
-    p.window = window;
-    p.sinks = sinks;
+    p.window = std::min(window, 1 << 30);      // more than all, and positions less it stay in range
+    p.sinks = std::min(sinks, 1 << 30);
     p.scale_log2 = sm_scale * 1.4426950408889634f;
     p.k_scale = kind == MD_KV_FP8_E4M3 ? k_scale : nullptr;
     p.v_scale = kind == MD_KV_FP8_E4M3 ? v_scale : nullptr;

@@ -148,6 +148,55 @@ def test_every_layout_of_the_work(ops, kind, name, D, H, KH, page, lens, rows, w
     check(f"{kind}/{name}", got, want, size, mx.attention_bound(size, q, values))
 
 
+# Four and eight wavefronts that share tiles, of every length, whole and in parts, pairs of request and kv head in eights and not: as above, by the
+# bounds.  (D, H, KH, page, requests, window, sinks, n_max, pages)
+SHARED = [
+    (64, 8, 8, 128, 3, 0, 0, 300, 40), (64, 4, 1, 128, 3, 0, 0, 300, 40), (64, 8, 2, 128, 3, 0, 0, 1100, 2), (64, 4, 1, 64, 5, 100, 3, 520, 2),
+    (64, 4, 1, 96, 3, 0, 0, 130, 300), (64, 8, 8, 96, 3, 100, 3, 520, 2), (64, 4, 1, 96, 9, 0, 0, 520, 2), (64, 4, 1, 32, 9, 100, 3, 520, 2),
+    (64, 4, 1, 128, 3, 0, 0, 100, 300), (64, 8, 8, 128, 5, 0, 0, 1100, 9), (64, 5, 5, 128, 3, 100, 3, 1100, 2), (64, 8, 8, 96, 3, 0, 0, 130, 300),
+    (64, 4, 1, 96, 9, 0, 0, 1100, 9), (64, 6, 3, 96, 3, 100, 3, 1100, 2), (128, 8, 8, 64, 3, 0, 0, 100, 40), (128, 4, 1, 128, 3, 0, 0, 300, 40),
+    (128, 8, 8, 128, 3, 0, 0, 1100, 2), (128, 4, 1, 64, 3, 100, 3, 40, 2), (128, 4, 1, 32, 3, 0, 0, 130, 300), (128, 8, 8, 96, 3, 100, 3, 520, 2),
+    (128, 4, 1, 32, 5, 0, 0, 520, 2), (128, 8, 8, 128, 3, 0, 0, 130, 40), (128, 4, 1, 128, 3, 0, 0, 100, 300), (128, 8, 2, 128, 3, 0, 0, 1100, 9),
+    (128, 5, 5, 128, 3, 100, 3, 1100, 2), (128, 4, 1, 64, 3, 0, 0, 100, 300), (128, 6, 3, 96, 5, 100, 3, 1100, 2), (128, 4, 1, 64, 9, 0, 0, 1100, 9),
+]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D,H,KH,page,B,window,sinks,n_max,most", SHARED)
+def test_tiles_shared_by_wavefronts(ops, kind, D, H, KH, page, B, window, sinks, n_max, most):
+    if kind in ("bf16", "fp8") and not window:
+        window = 1 << 20
+    lens = [[min(most * page - 5, 700), min(most * page, 333), 0, 40][b] if b < 4 else 1 + 13 * b for b in range(B)]
+    rows = [[min(n_max, lens[0], 290), min(n_max, 5), 0, 1][b] if b < 4 else b % 3 for b in range(B)]
+    tab = mx.table(lens, page, seed=D + n_max)
+    cache, scales, values = caches(kind, tab[3], KH, page, D, 5, ops)
+    q = (2 * torch.randn(sum(rows), H, D, generator=torch.Generator().manual_seed(1))).to(BF)
+    want, size = mx.window_attention(q, values, lens, rows, tab[0], tab[1], window, sinks)
+    out = attend(ops, q, cache, rows, lens, page, tab, window, sinks, scales, n_max=n_max, most=most)
+    check(f"{kind}/{D} {H}/{KH} pages of {page}, {B} x {n_max}", out, want, size, mx.attention_bound(size, q, values))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mxfp8"])
+@pytest.mark.parametrize("lens,rows", [([3, 130], [9, 2]), ([100, 0], [150, 60])])
+def test_the_largest_window_and_more_rows_than_tokens(ops, kind, lens, rows):
+    """A window and first tokens of 2^31 - 1 are all of them, for rows in front of a request's first token too, which see nothing."""
+    D, H, KH, page = 64, 4, 2, 128
+    tab = mx.table(lens, page)
+    cache, _, values = caches(kind, tab[3], KH, page, D, 5, ops)
+    q = torch.randn(sum(rows), H, D, generator=torch.Generator().manual_seed(1)).to(BF).to(DEV)
+    want, size = mx.window_attention(q.cpu(), values, lens, rows, tab[0], tab[1], 1 << 20, 0)
+    most, n = 2**31 - 1, max(rows)
+    lib, kind_ = ops._lib.load(), {"bf16": ops.MD_KV_BF16, "mxfp8": ops.MD_KV_MXFP8}[kind] | ops.MD_KV_LAYOUT_HND
+    indptr, table = mx.indptr_of(rows).to(DEV), [t.to(DEV) for t in tab[:3]]
+    for window, sinks in ((most, 0), (most, most), (5, most)):
+        ws = torch.zeros(lib.md_window_attn_workspace_bytes(len(lens), n, H, KH, D, tab[4], page, kind_, window, sinks), dtype=torch.uint8, device=DEV)
+        out = torch.full_like(q, 7.0)
+        assert lib.md_window_attn(q.data_ptr(), q.stride(0), cache.data_ptr(), out.data_ptr(), indptr.data_ptr(), *(t.data_ptr() for t in table),
+                                  len(lens), n, H, KH, D, page, window, sinks, 1 / math.sqrt(D), tab[4], kind_, None, None, ws.data_ptr(), ws.numel(),
+                                  torch.cuda.current_stream().cuda_stream) == 0
+        check(f"{kind}/window {window}, {sinks} first", out, want, size, mx.attention_bound(size, q.cpu(), values))
+
+
 @pytest.mark.parametrize("kind", ["bf16", "mxfp4"])
 @pytest.mark.parametrize("n", [1, 60])
 def test_rows_behind_the_last_request_stay(ops, kind, n):
