@@ -80,7 +80,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     const int per = (tiles.count + p.nsplit - 1) / p.nsplit;
     const int t_begin = split * per, t_end = min(tiles.count, t_begin + per);
 
-    const float sl2 = KIND == MD_KV_FP8_E4M3 ? p.scale_log2 * p.k_scale[kvh] : p.scale_log2;
+    // never 0, whatever the keys' scale: a hidden score is -infinity times it
+    const float sl2 = KIND == MD_KV_FP8_E4M3 ? fmaxf(p.scale_log2 * p.k_scale[kvh], 1.17549435e-38f) : p.scale_log2;
     const float vsc = KIND == MD_KV_FP8_E4M3 ? p.v_scale[kvh] : 1.0f;
     f32x4 o[QT][NB];
     float m[QT], l[QT];

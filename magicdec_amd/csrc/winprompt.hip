@@ -66,7 +66,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     auto sees = [&](int pos) { return pos <= hi && (p.window <= 0 || pos + KT - 1 > lo - p.window || pos < p.sinks); };
 
     bf16x8 qf[KS];
-    const float sl2 = KIND == MD_KV_FP8_E4M3 ? p.scale_log2 * p.k_scale[kvh] : p.scale_log2;
+    // never 0, whatever the keys' scale: a hidden score is -infinity times it
+    const float sl2 = KIND == MD_KV_FP8_E4M3 ? fmaxf(p.scale_log2 * p.k_scale[kvh], 1.17549435e-38f) : p.scale_log2;
     f32x16 o[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)

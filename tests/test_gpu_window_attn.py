@@ -238,6 +238,22 @@ def test_refusals_on_the_gpu(ops):
             op()
 
 
+@pytest.mark.parametrize("n,H", [(1, 2), (3, 8), (200, 4)])
+def test_scales_of_zero(ops, n, H):
+    """A static scale of 0, of a head whose first rows were all 0: keys and values of 0, so that a row is the mean of what it sees, and 0."""
+    D, KH, page, lens = 128, 2, 128, [300]
+    tab = mx.table(lens, page)
+    cache, (ks, vs), values = caches("fp8", tab[3], KH, page, D, 5, ops)
+    ks, vs = ks.clone(), vs.clone()
+    ks[0], vs[1] = 0.0, 0.0
+    values[:, 0, 0], values[:, 1, 1] = 0.0, 0.0
+    q = torch.randn(n, H, D, generator=torch.Generator().manual_seed(1)).to(BF)
+    want, size = mx.window_attention(q, values, lens, [n], tab[0], tab[1], 77, 3)
+    out = attend(ops, q, cache, [n], lens, page, tab, 77, 3, (ks, vs))
+    check(f"scales of 0, {n} rows", out, want, size, mx.attention_bound(size, q, values))
+    assert bool((out[:, H // 2:] == 0).all())
+
+
 def hidden_garbage(lens, rows, tab, page, window, sinks):
     """An edit of a cache that puts infinities, NaN and the largest numbers into every place that no row of the request sees."""
     indices, indptr = tab[0], tab[1]
