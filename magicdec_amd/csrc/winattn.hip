@@ -559,16 +559,17 @@ WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int p
     const int64_t keys = seen(pl.rows), have = pairs * pl.n_qgroups;
     if (rows <= 32) {
         // Keys over several workgroups, of enough keys each to pay for the launch that joins them (3.5).  One a CU up to half as many (4 x 4 rows over 5 000
-        // keys in bf16: 70 whole, 22 in 256, 25 in 512), two where 8- or 4-bit streams stay long (8 x 4 over 8 000 37 and 34); beyond that
-        // three where streams are long (32 x 4 over 9 000 120 whole, 110), and so where the last workgroups would leave CUs behind (40 x 4 over
-        // 9 000 in bf16 311 whole, 242 in three; 48 x 4 337 and 289 in two)
+        // keys in bf16: 70 whole, 22 in 256, 25 in 512), two where 8- or 4-bit streams stay long (8 x 4 over 8 000 37 and 34).  Up to a workgroup a
+        // CU three each where that is two a CU (130 over 8 000 keys of 64 in 4 bits 38 whole, 24; over 1 200 10.6 and 11.0), of 8- and 4-bit streams
+        // two beyond (200 over 8 000 in 8 bits 89 and 82, in bf16 143 and 156).  More workgroups: three where streams are long and the last ones
+        // would leave CUs behind (40 x 4 x 8 over 9 000 in bf16 311 whole, 242 in three; 48 x 4 x 8 337 and 289 in two)
         const int64_t stream = keys * 2 * kv_row_bytes(kind, D);
         const bool long_way = stream >= 700000, left = have * 100 < (have + 511) / 512 * 512 * 85;
         int64_t want;
         if (have <= 128)
             want = (kind != MD_KV_BF16 && keys * have >= 512000 ? 512 : 256) / have;
         else if (have <= 256)
-            want = kind != MD_KV_BF16 && long_way ? 768 / have : 1;
+            want = have * 3 <= 512 && keys >= 2048 ? 3 : kind != MD_KV_BF16 && keys >= 4096 ? 2 : 1;
         else
             want = !long_way || !left ? 1 : have <= 352 ? 3 : 2;
         pl.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, keys <= 512 ? 1 : keys / 128, 64}));
