@@ -178,7 +178,7 @@ int md_paged_attn(const void* q, int64_t q_row_stride, const void* cache, void* 
  *                     included, has no effect on the rows that it is hidden from.  sm_scale > 0; D 64 or 128.
  * workspace: md_window_attn_workspace_bytes(), 16-byte aligned, of this call alone until it has run.
  * ---------------------------------------------------------------------- */
-int md_kv_row_bytes(int kv_dtype, int D);
+size_t md_kv_row_bytes(int kv_dtype, int D);
 int md_read_paged_kv(void* k_out, void* v_out, int64_t k_row_stride, int64_t v_row_stride, const int32_t* indptr, const void* cache,
                      const int32_t* page_indices, const int32_t* page_indptr, const int32_t* last_page_len, int B, int n_max, int KH, int D,
                      int page_size, int kv_dtype, const float* k_scale, const float* v_scale, md_stream_t stream);

@@ -85,7 +85,7 @@ _SIGNATURES = {
     "md_debug_attn_timing": (None, [I, I]),
     "md_debug_attn_timing_read": (c_int, [P, I]),
     "md_paged_attn": (c_int, [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, c_float, I, I, P, P, P, c_size_t, P]),
-    "md_kv_row_bytes": (c_int, [I, I]),
+    "md_kv_row_bytes": (c_size_t, [I, I]),
     "md_read_paged_kv": (c_int, [P, P, L, L, P, P, P, P, P, I, I, I, I, I, I, P, P, P]),
     "md_window_attn_workspace_bytes": (c_size_t, [I, I, I, I, I, I, I, I, I, I]),
     "md_window_attn": (c_int, [P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, c_float, I, I, P, P, P, c_size_t, P]),

@@ -296,7 +296,7 @@ int md_mx_append(const void* q, const void* k, const void* v, int64_t qs, int64_
     return MD_OK;
 }
 
-extern "C" int md_kv_row_bytes(int kv_dtype, int D) {
+extern "C" size_t md_kv_row_bytes(int kv_dtype, int D) {
     const int kind = kv_dtype & MD_KV_DTYPE_MASK;
     return (D == 64 || D == 128) && kind <= MD_KV_MXFP4 ? kv_row_bytes(kind, D) : 0;
 }
