@@ -357,6 +357,8 @@ def paged_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page
 
     window: a row at position t sees the positions s <= t with s > t - window or s < sinks (None: all).  With a window, and over block-scaled
     caches (mx_kv_cache), the attention is causal."""
+    if (window is not None and window < 1) or sinks < 0:
+        raise ValueError(f"paged_attention: window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     if window is not None or _is_mx(kv_cache):
         return _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, n_max, max_pages_per_req, workspace, causal,
                                  sm_scale, out, kv_scales, kv_layout, window, sinks)
@@ -397,8 +399,6 @@ def _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_pa
         raise ValueError(f"{what}: attention with a window or over a block-scaled cache is causal")
     if H % KH or (width != D and not _is_mx(kv_cache)):
         raise ValueError(f"{what}: {H} query heads of {D} over {KH} kv heads of {width}")
-    if (window is not None and window < 1) or sinks < 0:
-        raise ValueError(f"{what}: window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     if out is None:
         out = torch.empty((rows, H, D), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
