@@ -175,7 +175,7 @@ int md_paged_attn(const void* q, int64_t q_row_stride, const void* cache, void* 
  *                     are left as they were.
  * md_window_attn      md_paged_attn (causal) of every kv_dtype, where a row at position t sees the positions s <= t with s > t - window or
  *                     s < sinks (window 0: all up to t).  A row that sees nothing is 0.  What is in a hidden place, infinities and NaN
- *                     included, has no effect on the rows that it is hidden from.  sm_scale > 0; D 64 or 128.  Per-head scales are not negative.
+ *                     included, has no effect on the rows that it is hidden from.  sm_scale > 0; D 64 or 128.  Per-head scales may be 0 or negative.
  * workspace: md_window_attn_workspace_bytes(), 16-byte aligned, of this call alone until it has run.
  * ---------------------------------------------------------------------- */
 size_t md_kv_row_bytes(int kv_dtype, int D);

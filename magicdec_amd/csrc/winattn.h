@@ -35,6 +35,14 @@ __device__ __forceinline__ int win_pair(const WinParams& p, int of, int& sub) {
 
 constexpr float kLowest = -3.402823466e38f;      // reference of a row without a key: finite, so that differences are no NaN
 
+// MD_KV_FP8_E4M3: the keys' scale is part of the scores' factor, which has to be above 0: a hidden score is -infinity times it, and the largest score is the
+// largest before it.  So its size goes there, and its sign to the queries.
+__device__ __forceinline__ float size_of_scale(float scale_log2, float k_scale) { return fmaxf(scale_log2 * fabsf(k_scale), 1.17549435e-38f); }
+__device__ __forceinline__ bf16x8 with_sign_of(float k_scale, bf16x8 q) {
+    const unsigned flip = k_scale < 0.f ? 0x80008000u : 0u;
+    return __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, q) ^ u32x4{flip, flip, flip, flip});
+}
+
 // Largest of lanes l and l ^ 16, of l and l ^ 32: swaps of 16 and of 32 lanes, no LDS
 __device__ __forceinline__ float max_over_16(float x) {
     const unsigned u = __builtin_bit_cast(unsigned, x);

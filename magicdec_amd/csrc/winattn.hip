@@ -85,8 +85,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
     const int per = (tiles.count + p.nsplit - 1) / p.nsplit;
     const int t_begin = split * per, t_end = min(tiles.count, t_begin + per);
 
-    // never 0, whatever the keys' scale: a hidden score is -infinity times it
-    const float sl2 = KIND == MD_KV_FP8_E4M3 ? fmaxf(p.scale_log2 * p.k_scale[kvh], 1.17549435e-38f) : p.scale_log2;
+    const float ksc = KIND == MD_KV_FP8_E4M3 ? p.k_scale[kvh] : 1.0f;
+    const float sl2 = KIND == MD_KV_FP8_E4M3 ? size_of_scale(p.scale_log2, ksc) : p.scale_log2;
     const float vsc = KIND == MD_KV_FP8_E4M3 ? p.v_scale[kvh] : 1.0f;
     f32x4 o[QT][NB];
     float m[QT], l[QT];
@@ -364,6 +364,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void window_attn_kernel(const WinPa
         for (int s = 0; s < KS; ++s) {
             const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
             qf[qt][s] = R < nrows ? *reinterpret_cast<const bf16x8*>(qp + (s / SPL) * 4 * EL + lc * EL + (s % SPL) * 8) : z;
+            if constexpr (KIND == MD_KV_FP8_E4M3) qf[qt][s] = with_sign_of(ksc, qf[qt][s]);
         }
     }
     // steady state: loads of the tile NS turns on are issued without a condition, so that waits are for the tile at hand alone

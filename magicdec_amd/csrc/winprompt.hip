@@ -73,8 +73,8 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
     auto sees = [&](int pos) { return pos <= hi && (p.window <= 0 || pos + KT - 1 > lo - p.window || pos < p.sinks); };
 
     bf16x8 qf[KS];
-    // never 0, whatever the keys' scale: a hidden score is -infinity times it
-    const float sl2 = KIND == MD_KV_FP8_E4M3 ? fmaxf(p.scale_log2 * p.k_scale[kvh], 1.17549435e-38f) : p.scale_log2;
+    const float ksc = KIND == MD_KV_FP8_E4M3 ? p.k_scale[kvh] : 1.0f;
+    const float sl2 = KIND == MD_KV_FP8_E4M3 ? size_of_scale(p.scale_log2, ksc) : p.scale_log2;
     f32x16 o[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db)
@@ -301,6 +301,7 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void window_prompt_kernel
         for (int ks = 0; ks < KS; ++ks) {
             const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
             qf[ks] = valid ? *reinterpret_cast<const bf16x8*>(qp + ks * 16 + kh * 8) : z;
+            if constexpr (KIND == MD_KV_FP8_E4M3) qf[ks] = with_sign_of(ksc, qf[ks]);
         }
     }
     for (int i = t_begin; i < t_end; ++i) {
