@@ -93,6 +93,18 @@ def _rows_of(what, t, heads, D):
     return n
 
 
+def _share_memory(a, b):
+    """Do two tensors of rows [rows, heads, D] (as _rows_of has them, each row's elements dense) have an element in common?"""
+    d = (b.data_ptr() - a.data_ptr()) // 2
+    first, second = (a, b) if d >= 0 else (b, a)
+    d, n, width, s = abs(d), first.shape[0], first.shape[1] * first.shape[2], first.stride(0)
+    if d >= (n - 1) * s + width:
+        return False
+    if n == 1 or s != second.stride(0):
+        return True                                   # (rows of unequal distance may pass one another: not asked any closer)
+    return d % s < width or s - d % s < second.shape[1] * second.shape[2]
+
+
 def _table_of(what, indptr, page_indices, page_indptr, last_page_len, offsets=None):
     """How many requests a page table, with the rows' indptr and offsets, has: int32, contiguous."""
     for t in (indptr, page_indices, page_indptr, last_page_len):
@@ -219,6 +231,8 @@ def read_kv(k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_las
         raise ValueError(f"{what}: rows of {D} elements of a cache of {width}")
     if rows > 1 and min(k.stride(0), v.stride(0)) < KH * D:
         raise ValueError(f"{what}: k and v are written: rows that share memory")
+    if rows and _share_memory(k, v):
+        raise ValueError(f"{what}: k and v are written: they share memory")
     if B >= 1 and rows:
         check(_lib.load().md_read_paged_kv(k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), indptr.data_ptr(), kv_cache.data_ptr(),
                                            _pages(kv_page_indices, kv_page_indptr), kv_page_indptr.data_ptr(), kv_page_lastlen.data_ptr(), B,

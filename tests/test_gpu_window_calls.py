@@ -32,3 +32,21 @@ def test_negative_scales_of_heads(ops, D, n, H):
         want, size = mx.window_attention(q, values, lens, [n], tab[0], tab[1], window, sinks)
         out = attend(ops, q, cache, [n], lens, page, tab, window, sinks, (ks, vs))
         check(f"negative scales, {n} rows, window {window}", out, want, size, mx.attention_bound(size, q, values))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mxfp8"])
+def test_read_kv_refuses_one_place_for_keys_and_values(ops, kind):
+    """k and v are written by many workgroups in no order; slices of one buffer whose rows lie between each other's are two places."""
+    D, KH, page, n = 64, 2, 128, 5
+    cache = ops.mx_kv_cache(1, KH, D, kind) if kind != "bf16" else torch.zeros(1, 2, KH, page, D, dtype=BF, device=DEV)
+    table = [torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, n], [0], [0, 1], [n])]
+    x = (torch.arange(n * 2 * KH * D) % 13).to(BF).view(n, 2 * KH, D).to(DEV)
+    ops.update_kv(x[:, :KH], x[:, KH:], table[0], cache, *table[1:], kv_layout="HND")
+    both = torch.zeros(n + 1, 2 * KH, D, dtype=BF, device=DEV)
+    out = both[:n, :KH]
+    for v in (out, both[:n, 1:KH + 1], both[1:, :KH]):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.read_kv(out, v, table[0], cache, *table[1:], kv_layout="HND")
+    assert bool((both == 0).all())
+    ops.read_kv(out, both[:n, KH:], table[0], cache, *table[1:], kv_layout="HND")
+    assert torch.equal(both[:n], x) and bool((both[n] == 0).all())

@@ -15,3 +15,22 @@ def test_windows_and_first_tokens_out_of_range(kind, window, sinks):
     q, i = torch.zeros(1, 2, 64, dtype=BF), torch.zeros(2, dtype=torch.int32)
     with pytest.raises(ValueError, match="window must be at least 1 and sinks at least 0"):
         ops.paged_attention(q, cache, i, i, i, i, 1, 1, None, kv_layout="HND", window=window, sinks=sinks)
+
+
+def test_rows_that_are_written_twice_are_found():
+    """Two tensors of rows in one buffer, against the sets of their elements; rows of unequal distance whose ranges meet count as shared."""
+    heads, D, at = 2, 8, torch.arange(2000)
+    buffer = torch.zeros(2000, dtype=BF)
+    seen = set()
+    for n in (1, 2, 3):
+        for stride in (16, 24, 32, 40):
+            for other in {stride, 24}:
+                for d in range(0, 160, 8):
+                    k, v = (torch.as_strided(buffer, (n, heads, D), (s, D, 1), o) for s, o in ((stride, 0), (other, d)))
+                    places = [set(torch.as_strided(at, (n, heads, D), (s, D, 1), o).flatten().tolist()) for s, o in ((stride, 0), (other, d))]
+                    common = bool(places[0] & places[1])
+                    for a, b in ((k, v), (v, k)):
+                        got = ops._share_memory(a, b)
+                        assert got == common or (got and n > 1 and stride != other), (n, stride, other, d)
+                    seen.add((common, n))
+    assert len(seen) == 6
