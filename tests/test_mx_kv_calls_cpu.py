@@ -34,3 +34,36 @@ def test_rows_that_are_written_twice_are_found():
                         assert got == common or (got and n > 1 and stride != other), (n, stride, other, d)
                     seen.add((common, n))
     assert len(seen) == 6
+
+
+class OnDevice:
+    """A CPU tensor that says it is on a GPU."""
+
+    def __init__(self, t, index):
+        self.t, self.index, self.is_cuda, self.device = t, index, True, f"cuda:{index}"
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return self.index
+
+
+@pytest.mark.parametrize("call", ["read_kv", "paged_attention"])
+def test_scales_of_another_device_are_refused(call, monkeypatch):
+    """The kernels read a static-scale cache's scales on the current device, as all else."""
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(ops._lib, "load", lambda: pytest.fail("the library was called"))
+    KH, D = 2, 64
+    here = lambda t: OnDevice(t, 0)  # noqa: E731
+    cache = here(torch.zeros(1, 2, KH, 128, D).to(ops.FP8_DTYPE))
+    rows = [here(torch.zeros(1, KH, D, dtype=BF)) for _ in (0, 1)]
+    i = here(torch.tensor([0, 1], dtype=torch.int32))
+    for other in (0, 1):
+        scales = [here(torch.ones(KH)) for _ in (0, 1)]
+        scales[other] = OnDevice(torch.ones(KH), 1)
+        with pytest.raises(ValueError, match="cuda:1"):
+            if call == "read_kv":
+                ops.read_kv(*rows, i, cache, i, i, i, kv_scales=tuple(scales), kv_layout="HND")
+            else:
+                ops.paged_attention(rows[0], cache, i, i, i, i, 1, 1, None, kv_scales=tuple(scales), kv_layout="HND", window=5)
