@@ -42,6 +42,10 @@ void md_debug_set_fused_split(int S);
 void md_debug_set_tile_timing(void* buf);
 /* md_linear_block: workgroups to aim for when K is split (0 = default 256); non-temporal weight DMA (1 = default) */
 void md_debug_set_block_gemm(int target_blocks, int weights_nontemporal);
+/* md_window_attn, md_window_attn_workspace_bytes: where each of the next calls writes how it lays out its rows and keys, five numbers of host memory:
+ * wavefronts that share tiles (0: the kernel of few rows), query rows of a workgroup, row groups of a request and kv head, parts of their keys, keys of a
+ * tile; NULL = off */
+void md_debug_set_window_report(int* report);
 
 #ifdef __cplusplus
 }

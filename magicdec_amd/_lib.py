@@ -190,6 +190,7 @@ _DEV_SIGNATURES = {
     "md_debug_set_fused_split": (None, [I]),
     "md_debug_set_tile_timing": (None, [P]),
     "md_debug_set_block_gemm": (None, [I, I]),
+    "md_debug_set_window_report": (None, [P]),
 }
 DEV_SYMBOLS = tuple(_DEV_SIGNATURES)
 

@@ -124,7 +124,11 @@ struct PageCursor {
     __device__ __forceinline__ int64_t id() const { return __builtin_amdgcn_readlane(ids, page - base); }
 };
 
-// winprompt.hip, an object each: calls of more than 32 rows, in workgroups of nw (4 or 8) wavefronts of 32
+// winprompt.hip, an object each: calls of more than 32 rows, in workgroups of nw (4 or 8) wavefronts of 32, on tiles of as many keys as divide a page
+inline int window_prompt_tile(int D, int nw, int page_size) {
+    const int keys = D == 128 && nw == 8 ? 128 : 64;
+    return page_size % keys == 0 ? keys : 32;
+}
 int md_window_prompt_0(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_BF16
 int md_window_prompt_1(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_FP8_E4M3
 int md_window_prompt_2(const WinParams& p, int D, int nw, int grid, hipStream_t st);      // MD_KV_MXFP8

@@ -524,6 +524,8 @@ struct WinWay {
     }
 };
 
+int* g_report = nullptr;       // dev knob (md_debug_set_window_report)
+
 // All in us, 8 kv heads unless said.
 WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int page_size, int kind, int window, int sinks) {
     WinPlan pl;
@@ -579,6 +581,10 @@ WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int p
     // -> 12.2; one request of 1 500 in eight parts 8.5 -> 9.9
     pl.kg = kind == MD_KV_MXFP4 && D == 64 && pl.rows == 16 && page_size % 64 == 0 && keys / pl.nsplit >= 1024 ? 2 : 1;
     pl.slots = pl.nsplit > 1 ? (size_t)have * pl.nsplit * pl.rows : 0;
+    if (g_report) {
+        const int report[5] = {pl.nw, pl.rows, pl.n_qgroups, pl.nsplit, pl.nw ? window_prompt_tile(D, pl.nw, page_size) : 32 * pl.kg};
+        std::copy(report, report + 5, g_report);
+    }
     return pl;
 }
 
@@ -645,6 +651,10 @@ bool window_shape_ok(int B, int n_max, int H, int KH, int max_pages, int page_si
 }
 
 }  // namespace
+
+#ifdef MD_DEV_KNOBS   // include/magicdec_hip_dev.h: not part of the drop-in boundary
+extern "C" void md_debug_set_window_report(int* report) { g_report = report; }
+#endif
 
 extern "C" size_t md_window_attn_workspace_bytes(int B, int n_max, int H, int KH, int D, int max_pages_per_req, int page_size, int kv_dtype,
                                                  int window, int sinks) {

@@ -388,12 +388,12 @@ int launch_prompt(const WinParams& p, int grid, hipStream_t st) {
 #define MD_WIN_CAT_(a, b) a##b
 #define MD_WIN_CAT(a, b) MD_WIN_CAT_(a, b)
 
-// tiles never cross a page: as many keys as divide it
 int MD_WIN_CAT(md_window_prompt_, MD_WIN_KIND)(const WinParams& p, int D, int nw, int grid, hipStream_t st) {
+    const bool small = window_prompt_tile(D, nw, p.page_size) == 32;
     if (D == 128) {
-        if (nw == 8) return p.page_size % 128 == 0 ? launch_prompt<128, 8, 128>(p, grid, st) : launch_prompt<128, 8, 32>(p, grid, st);
-        return p.page_size % 64 == 0 ? launch_prompt<128, 4, 64>(p, grid, st) : launch_prompt<128, 4, 32>(p, grid, st);
+        if (nw == 8) return small ? launch_prompt<128, 8, 32>(p, grid, st) : launch_prompt<128, 8, 128>(p, grid, st);
+        return small ? launch_prompt<128, 4, 32>(p, grid, st) : launch_prompt<128, 4, 64>(p, grid, st);
     }
-    if (nw == 8) return p.page_size % 64 == 0 ? launch_prompt<64, 8, 64>(p, grid, st) : launch_prompt<64, 8, 32>(p, grid, st);
-    return p.page_size % 64 == 0 ? launch_prompt<64, 4, 64>(p, grid, st) : launch_prompt<64, 4, 32>(p, grid, st);
+    if (nw == 8) return small ? launch_prompt<64, 8, 32>(p, grid, st) : launch_prompt<64, 8, 64>(p, grid, st);
+    return small ? launch_prompt<64, 4, 32>(p, grid, st) : launch_prompt<64, 4, 64>(p, grid, st);
 }
