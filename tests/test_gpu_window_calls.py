@@ -50,3 +50,36 @@ def test_read_kv_refuses_one_place_for_keys_and_values(ops, kind):
     assert bool((both == 0).all())
     ops.read_kv(out, both[:n, KH:], table[0], cache, *table[1:], kv_layout="HND")
     assert torch.equal(both[:n], x) and bool((both[n] == 0).all())
+
+
+@pytest.mark.parametrize("kind", ["bf16", "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("window,sinks", [(50, 3), (0, 0)])
+def test_each_request_of_a_batch_by_itself(ops, kind, window, sinks):
+    """A batch as large as to split no keys, and its requests one a call: the same bits where their keys are in one part there too (a window of few keys);
+    otherwise, in up to five parts, both within the bound of 64 bits."""
+    from tests import window_layouts as wl
+    D, H, KH, page = 128, 8, 8, 128
+    lens, rows = [100 + 7 * b for b in range(64)], [1 + b % 4 for b in range(64)]
+    indices, indptr, last, pages, most = mx.table(lens, page)
+    cache, _, values = caches(kind, pages, KH, page, D, 5, ops)
+    q = torch.randn(sum(rows), H, D, generator=torch.Generator().manual_seed(1)).to(BF)
+    window = wl.window_of(window, kind)
+    want, size = mx.window_attention(q, values, lens, rows, indices, indptr, window, sinks)
+    bound = mx.attention_bound(size, q, values)
+    ws = ops.AttnWorkspace(DEV)
+    at, parts = mx.indptr_of(rows).tolist(), set()
+    with wl.reported(ops._lib.load()) as layout:
+        whole = attend(ops, q, cache, rows, lens, page, (indices, indptr, last, pages, most), window, sinks, ws=ws)
+        of_batch = layout()
+        check(f"{kind}/64 requests", whole, want, size, bound)
+        for b in range(64):
+            mine = slice(at[b], at[b + 1])
+            tab = (indices[int(indptr[b]):int(indptr[b + 1])], torch.tensor([0, int(indptr[b + 1] - indptr[b])], dtype=torch.int32), last[b:b + 1], 0, most)
+            alone = attend(ops, q[mine], cache, rows[b:b + 1], lens[b:b + 1], page, tab, window, sinks, ws=ws)
+            parts.add(layout())
+            if window == 50:
+                assert torch.equal(alone, whole[mine])
+            else:
+                assert bool(((alone.cpu().double() - want[mine]).abs() <= bound[mine]).all()), b
+    if of_batch is not None:
+        assert of_batch == (0, 16, 32, "whole") and parts == {(0, 16, 32, "whole" if window == 50 else "few")}
