@@ -83,3 +83,40 @@ def test_each_request_of_a_batch_by_itself(ops, kind, window, sinks):
                 assert bool(((alone.cpu().double() - want[mine]).abs() <= bound[mine]).all()), b
     if of_batch is not None:
         assert of_batch == (0, 16, 32, "whole") and parts == {(0, 16, 32, "whole" if window == 50 else "few")}
+
+
+# (D, H, KH, requests, n_max, wavefronts that share tiles): pages of 32 rows, so that a part walks more of them than a wavefront holds numbers of
+LONG = [(64, 1, 1, 520, 1, 0), (128, 1, 1, 520, 1, 0), (64, 4, 1, 520, 8, 0), (128, 4, 1, 520, 8, 0), (64, 2, 1, 160, 150, 4), (64, 4, 1, 80, 400, 8),
+        (128, 2, 1, 160, 150, 4), (128, 4, 1, 80, 400, 8)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "mxfp8", "mxfp4"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (2960, 70), (2300, 2100)])
+@pytest.mark.parametrize("D,H,KH,B,n_max,nw", LONG, ids=[f"{c[0]}-{c[5]}-waves-{c[4]}-rows" for c in LONG])
+def test_streams_of_more_pages_than_a_wavefront_holds_numbers_of(ops, kind, window, sinks, D, H, KH, B, n_max, nw):
+    """A request of 157 pages among short ones, whole or in two parts, with infinities and NaN in front of its window: where they are hidden from some row of
+    a tile, the wavefronts go back to that tile's page."""
+    from tests import window_layouts as wl
+    page, n = 32, 5000
+    window = wl.window_of(window, kind)
+    new = min(n_max, 70)
+    lens, rows = [n, 1, 40, 7] + [0] * (B - 4), [new, 1, 0, 2] + [0] * (B - 4)
+    tab = mx.table(lens, page, seed=3)
+    first = n - new                                           # the first row's position
+    seen = torch.arange(n) <= n - 1
+    if window:
+        seen &= (torch.arange(n) > first - window) | (torch.arange(n) < sinks)
+
+    def edit(x):
+        junk = torch.tensor([float("nan"), float("inf"), float("-inf"), 3.3895313892515355e38]).to(BF).repeat(D // 4)
+        for pos in (~seen).nonzero().flatten().tolist():
+            x[int(tab[0][pos // page]), :, :, pos % page] = junk
+    cache, scales, _ = caches(kind, tab[3], KH, page, D, 5, ops, edit=edit)
+    _, _, values = caches(kind, tab[3], KH, page, D, 5, ops)
+    q = torch.randn(sum(rows), H, D, generator=torch.Generator().manual_seed(1)).to(BF)
+    want, size = mx.window_attention(q, values, lens, rows, tab[0], tab[1], window, sinks)
+    with wl.reported(ops._lib.load()) as layout:
+        out = attend(ops, q, cache, rows, lens, page, tab, window, sinks, scales, n_max=n_max)
+        took = layout()
+    check(f"{kind}/157 pages, {nw} wavefronts, window {window}", out, want, size, mx.attention_bound(size, q, values))
+    assert took is None or (took[0] == nw and took[3] in ("whole", "few")), took
