@@ -14,7 +14,7 @@
 // whose elements and scales lie side by side in a page, so that no line is written from two XCDs' caches but at a workgroup's ends.
 //
 // 64 x 128 rows of 32 + 8 + 8 heads of 128, rotated and quantised to 4 bits, take 31 us (177 MB in and out, 5.7 TB/s) and 9 to read back; 8 x 16 032 rows of 4-bit
-// pages read back 131 us (665 MB, 5.0 TB/s: what a copy reaches); 256 rows 3.9 and 3.0, a launch's length.
+// pages read back 131 us (665 MB, 5.0 TB/s: what a copy reaches); 256 rows 4.0 and 2.9, a launch's length.
 #include "kvpages.h"
 
 #include <algorithm>

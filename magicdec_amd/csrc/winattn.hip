@@ -17,10 +17,10 @@
 // a NaN: in tiles that hide a key from some row, such values are taken out of the image, and what rows that do see them get of them is
 // added by itself (`spread`), from a second and third image of their signs.
 //
-// Long streams are bound by memory: 64 requests of 16 036 keys x 16 rows (8 heads of 128) take 331 us from 8-bit pages (2.2 GB, 6.6 TB/s; loads alone
-// 328) and 182 from 4-bit ones (1.1 GB, 6.1 TB/s), vector instructions in 26 and 45 % of the cycles, the matrix
+// Long streams are bound by memory: 64 requests of 16 036 keys x 16 rows (8 heads of 128) take 330 us from 8-bit pages (2.2 GB, 6.6 TB/s; loads alone
+// 328) and 184 from 4-bit ones (1.1 GB, 6.1 TB/s), vector instructions in 26 and 45 % of the cycles, the matrix
 // cores in 8 and 16.  Short ones by the way through a workgroup, its page numbers, keys, sums and rows one behind the other: 64 requests that see 257 keys
-// of 64 in bf16 11.5 us (34 MB), one of 32 065 keys 13 and 3 for the launch that joins its 32 parts.
+// of 64 in bf16 11.5 us (34 MB), one of 32 065 keys 13 and 4 for the launch that joins its 32 parts.
 #include "winattn.h"
 
 #include <algorithm>
@@ -526,7 +526,8 @@ struct WinWay {
 
 int* g_report = nullptr;       // dev knob (md_debug_set_window_report)
 
-// All in us, 8 kv heads unless said.
+// All in us, 8 kv heads unless said.  The bounds alone are known here, not the rows: one request's many choose the layout of all (63 requests of one token behind 16 032
+// and one of 128 in 8 bits 1 439; in a call each 324 and 55).
 WinPlan window_plan(int B, int n_max, int H, int KH, int D, int max_pages, int page_size, int kind, int window, int sinks) {
     WinPlan pl;
     const int64_t rows = (int64_t)n_max * (H / KH), pairs = (int64_t)B * KH;

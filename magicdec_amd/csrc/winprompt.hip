@@ -10,9 +10,9 @@
 //
 // Infinite values and NaN in tiles that hide a key from some row: as in winattn.hip, by all wavefronts together.
 //
-// 128 rows a request x 16 requests behind 16 032 keys (8-bit pages, 4 query heads of 128 on each of 8) take 549 us, 984 TFLOP/s: matrix cores and vector
+// 128 rows a request x 16 requests behind 16 032 keys (8-bit pages, 4 query heads of 128 on each of 8) take 550 to 557 us, 975 TFLOP/s: matrix cores and vector
 // instructions each in 46 % of the cycles, mostly in turn, at 2.0 GHz (the power limit; a library product of 8 192^3 reaches 1 189).  Prompts of 2 x 4 133
-// tokens with a window of 1 024 199 us, 612 TFLOP/s of the weights that count: a tenth more keys than a group's windows hold, and the first tile of each of
+// tokens with a window of 1 024 196 to 204 us, 610 TFLOP/s of the weights that count: a tenth more keys than a group's windows hold, and the first tile of each of
 // four rounds of workgroups, one a CU (eight wavefronts of 256 registers, 137 KB of images).  Tiles of 32-key blocks (555 -> 610), masked and unmasked
 // tiles in a body each (spills), two tiles in flight (bf16 to 1.5 times the time) and half of the wavefronts half a tile behind the others, so that
 // one's products run beside the other's exponentials (545 -> 575 to 620), were slower.

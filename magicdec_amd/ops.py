@@ -69,7 +69,7 @@ def _is_mx(kv_cache):
 
 # The checks of calls that a step makes: attributes of a tensor that cost least, each asked for once.  A step's calls are as short for the GPU as
 # they are for the host (append and read_kv of 256 rows: 7 us of kernels; 46 us of the host with torch.cuda.current_stream, shapes and
-# ctypes objects for every argument, 25 so).
+# ctypes objects for every argument, 26 so).
 def _here(what, first, *ts):
     """The current device, on which all these tensors (or None) have to be: the kernels run on its current stream."""
     if not first.is_cuda:
@@ -125,7 +125,7 @@ def _pages(page_indices, page_indptr):
 
 def _kv_args(kv_cache, kv_scales, kv_layout="NHD", head_dim=None):
     """(kv_dtype | layout flag, k_scale ptr, v_scale ptr) for a paged cache: bf16 caches take no scales, e4m3fn
-    caches need per-kv-head float32 dequantisation scales `(k_scale[KH], v_scale[KH])`; block-scaled ones (uint8) hold theirs, and their
+    caches need per-kv-head float32 dequantisation scales `(k_scale[KH], v_scale[KH])`, keys' above 0 where there is no window; block-scaled ones (uint8) hold theirs, and their
     rows' bytes with head_dim say which of the two they are."""
     flag = MD_KV_LAYOUT_HND if kv_layout == "HND" else 0
     if _is_mx(kv_cache):
@@ -370,7 +370,7 @@ def paged_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page
     plan() arguments passed explicitly.
 
     window: a row at position t sees the positions s <= t with s > t - window or s < sinks (None: all).  With a window, and over block-scaled
-    caches (mx_kv_cache), the attention is causal."""
+    caches (mx_kv_cache), the attention is causal; with a window kv_scales may be 0 or negative, keys' otherwise have to be above 0."""
     if (window is not None and window < 1) or sinks < 0:
         raise ValueError(f"paged_attention: window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     if window is not None or _is_mx(kv_cache):
