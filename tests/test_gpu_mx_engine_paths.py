@@ -186,3 +186,32 @@ def test_tensor_parallel_shards(ckpt, ids, kind):
         assert differ <= 0.02
     eng.inference(ids[:, :gc.GAMMA + 1].clone())
     assert off(torch.cat([rank["logits"] for rank in ranks], 1), eng.model._last_logits.cpu()) <= OFF[kind]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("name,streaming", [("tiny70b", False), ("tinyqwen", False), ("tinytgt", True), ("tiny70b", True)])
+def test_self_speculation_of_other_models(ckpt, ids, kind, name, streaming):
+    """Eight query heads of 128 on a kv head, five of 64, and the StreamingLLM draft beside a block-scaled verify cache: a verify step's logits near those over
+    16-bit pages, and a whole run with captured steps the run without, token for token."""
+    from magicdec_amd import harness
+    from magicdec_amd.Engine.StreamingLLM.backend import LMBackend as Streaming
+    logits, runs = {}, []
+    for kv, graphs in (("bf16", False), (kind, False), (kind, True)):
+        if streaming:
+            eng = Streaming(dtype=BF, device=DEV, dec_len=gc.GAMMA + 1)
+            eng.load_model(ckpt / name / "model.pth", use_tp=False)
+            if graphs:
+                eng.compile()
+            eng.setup_caches(max_batch_size=gc.B, max_seq_length=gc.MAX_LEN, draft_budget=gc.BUDGET, kv_dtype=kv)
+        else:
+            eng = target(ckpt / name, kv, graphs, draft_budget=gc.BUDGET)
+        eng.encode(ids)
+        eng.verify(ids[:, :gc.GAMMA + 1].clone())
+        logits[kv] = eng.model._last_logits.float().cpu()
+        st, _ = harness.run_selfspec_batch(eng, ids, gc.GAMMA, gc.MAX_LEN, gc.EOT_1, gc.EOT_2, streaming)
+        assert st.iters > 3 and bool((st.num_nodes.cpu() > ids.shape[1]).all())
+        if kv == kind:
+            runs.append((st.output.cpu(), st.num_nodes.cpu(), eng.cachelens.cpu()))
+    assert 0 < off(logits[kind], logits["bf16"]) <= OFF[kind]
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
