@@ -220,7 +220,7 @@ def read_kv(k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_las
     of k and v [rows, KH, D] (in place; returns them).  Rows of positions in front of a request's first token or outside its pages stay as they
     were.  n_max: the most rows of a request (None: as many as there are rows)."""
     what = "read_kv"
-    cur = _here(what, k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, *(kv_scales or ()))
+    cur = _here(what, k, v, indptr, kv_cache, kv_page_indices, kv_page_indptr, kv_page_lastlen, *(() if kv_scales is None else kv_scales))
     page_size, KH, width = _kv_geom(kv_cache, kv_layout)
     D = k.shape[-1]
     kind, ks, vs = _kv_args(kv_cache, kv_scales, kv_layout, D)
@@ -404,7 +404,7 @@ def _window_workspace(*shape):
 def _window_attention(q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, n_max, max_pages_per_req, workspace, causal, sm_scale, out,
                       kv_scales, kv_layout, window, sinks):
     what = "paged_attention"
-    cur = _here(what, q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, out, *(kv_scales or ()))
+    cur = _here(what, q, kv_cache, qo_indptr, page_indices, page_indptr, last_page_len, out, *(() if kv_scales is None else kv_scales))
     page_size, KH, width = _kv_geom(kv_cache, kv_layout)
     _, H, D = q.shape
     kind, ks, vs = _kv_args(kv_cache, kv_scales, kv_layout, D)

@@ -120,3 +120,18 @@ def test_streams_of_more_pages_than_a_wavefront_holds_numbers_of(ops, kind, wind
         took = layout()
     check(f"{kind}/157 pages, {nw} wavefronts, window {window}", out, want, size, mx.attention_bound(size, q, values))
     assert took is None or (took[0] == nw and took[3] in ("whole", "few")), took
+
+
+def test_scales_in_one_tensor(ops):
+    """kv_scales is two tensors: a tuple's, or the rows of one of [2, heads]."""
+    D, H, KH, page, lens, n = 128, 4, 2, 128, [300], 3
+    tab = mx.table(lens, page)
+    cache, scales, _ = caches("fp8", tab[3], KH, page, D, 5, ops)
+    q = torch.randn(n, H, D, generator=torch.Generator().manual_seed(1)).to(BF)
+    table = [t.to(DEV) for t in (mx.indptr_of([n]), *tab[:3])]
+    outs, rows = [], []
+    for s in (scales, torch.stack(scales)):
+        outs.append(attend(ops, q, cache, [n], lens, page, tab, 77, 3, s))
+        k, v = (torch.zeros(n, KH, D, dtype=BF, device=DEV) for _ in (0, 1))
+        rows.append(torch.cat(ops.read_kv(k, v, table[0], cache, *table[1:], n_max=n, kv_scales=s, kv_layout="HND")))
+    assert torch.equal(*outs) and torch.equal(*rows) and bool(rows[0].any())
