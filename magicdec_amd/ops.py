@@ -125,8 +125,8 @@ def _pages(page_indices, page_indptr):
 
 def _kv_args(kv_cache, kv_scales, kv_layout="NHD", head_dim=None):
     """(kv_dtype | layout flag, k_scale ptr, v_scale ptr) for a paged cache: bf16 caches take no scales, e4m3fn
-    caches need per-kv-head float32 dequantisation scales `(k_scale[KH], v_scale[KH])`, keys' above 0 where there is no window; block-scaled ones (uint8) hold theirs, and their
-    rows' bytes with head_dim say which of the two they are."""
+    caches need per-kv-head float32 dequantisation scales `(k_scale[KH], v_scale[KH])`, the keys' above 0 for attention without a window;
+    block-scaled ones (uint8) hold theirs, and their rows' bytes with head_dim say which of the two they are."""
     flag = MD_KV_LAYOUT_HND if kv_layout == "HND" else 0
     if _is_mx(kv_cache):
         if kv_layout != "HND" or kv_scales is not None:
