@@ -58,9 +58,9 @@ def test_each_request_of_a_batch_by_itself(ops, kind, window, sinks):
     """A batch as large as to split no keys, and its requests one a call: the same bits where their keys are in one part there too (a window of few keys);
     otherwise, in up to five parts, both within the bound of 64 bits."""
     from tests import window_layouts as wl
-    D, H, KH, page = 128, 8, 8, 128
-    lens, rows = [100 + 7 * b for b in range(64)], [1 + b % 4 for b in range(64)]
-    indices, indptr, last, pages, most = mx.table(lens, page)
+    D, H, KH, page, most = 64, 2, 2, 64, 10
+    lens, rows = [100 + 2 * b for b in range(130)], [1 + b % 4 for b in range(130)]
+    indices, indptr, last, pages, _ = mx.table(lens, page)
     cache, _, values = caches(kind, pages, KH, page, D, 5, ops)
     q = torch.randn(sum(rows), H, D, generator=torch.Generator().manual_seed(1)).to(BF)
     window = wl.window_of(window, kind)
@@ -71,8 +71,8 @@ def test_each_request_of_a_batch_by_itself(ops, kind, window, sinks):
     with wl.reported(ops._lib.load()) as layout:
         whole = attend(ops, q, cache, rows, lens, page, (indices, indptr, last, pages, most), window, sinks, ws=ws)
         of_batch = layout()
-        check(f"{kind}/64 requests", whole, want, size, bound)
-        for b in range(64):
+        check(f"{kind}/130 requests", whole, want, size, bound)
+        for b in range(130):
             mine = slice(at[b], at[b + 1])
             tab = (indices[int(indptr[b]):int(indptr[b + 1])], torch.tensor([0, int(indptr[b + 1] - indptr[b])], dtype=torch.int32), last[b:b + 1], 0, most)
             alone = attend(ops, q[mine], cache, rows[b:b + 1], lens[b:b + 1], page, tab, window, sinks, ws=ws)
